@@ -83,6 +83,9 @@ def _compile_cmds() -> List[tuple]:
     hip_flags = [
         hipcc, "-O3", "-std=c++17", f"--offload-arch={ARCH}", "-fPIC",
         "-munsafe-fp-atomics", f"-I{CSRC}",
+        # no packed fp32 (v_pk_add / mul / fma_f32): -O3 forms them from ordinary float code, and some of their
+        # operand forms have given wrong results on MI355X now and then, with no error
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     ] + os.environ.get("DTA_HIP_EXTRA_FLAGS", "").split()  # e.g. -DDTA_MP_PHASES (diagnostic builds)
     cxx = os.environ.get("CXX", "g++")
     cpp_flags = [
