@@ -1065,9 +1065,11 @@ std::shared_ptr<MlpPersistentLaunch> mlp_persistent_prepare(
 }
 
 void dta_register_ext(pybind11::module_& m);
+void dta_register_pref(pybind11::module_& m);
 
 PYBIND11_MODULE(_C, m) {
   dta_register_ext(m);
+  dta_register_pref(m);
   m.doc() = "distributed_training_amd native runtime (gfx950 HIP kernels + RCCL communicator)";
   m.def("flat_sgd", &flat_sgd);
   m.def("flat_adam", &flat_adam, py::arg("p"), py::arg("g"), py::arg("m"), py::arg("v"), py::arg("vmax"),

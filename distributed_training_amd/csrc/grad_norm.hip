@@ -1,0 +1,245 @@
+// Global 2-norm of many gradient tensors, and clipping by it.
+//
+//   norm = sqrt(sum_t sum_i g_t[i]^2),   g_t[i] *= min(1, max_norm / (norm + 1e-6))
+//
+// Bound by memory: one read of every gradient for the norm, one more read and a write when it clips.
+// The tensors of a call lie anywhere and have any type and size, so the work is cut into units of kUnit
+// elements numbered over all tensors, and every workgroup takes one run of consecutive units: equal shares
+// whatever the sizes are, one search for the first tensor and a step to the next where a run crosses over.
+// The tensors' addresses travel in the launch's arguments (kJobs of them a launch, no table in device memory to
+// fill, so a launch can be captured).
+//
+// Squares are summed in 64 bits: fp64 has the rate of unpacked fp32 here and the pass waits for memory, so it
+// costs nothing; the squares of gradients near 1e20 or 1e-25 neither overflow nor vanish.  Each workgroup leaves
+// one partial sum, and one workgroup adds the partials in a fixed order: no atomics, the same bits every call.
+#include "common.h"
+
+namespace dta {
+
+constexpr int kJobs = 160;     // 160 x 20 B of arguments stay under 4 KiB
+constexpr int kUnit = 8192;    // elements: 4 (2 bytes) to 16 (8 bytes) 16-byte loads a thread
+constexpr int kNormGrid = 2048;  // 8 workgroups on each of 256 CUs
+
+struct NormJobs {
+  int n;
+  int units;               // of this launch
+  int start[kJobs + 1];    // first unit of each tensor
+  void* p[kJobs];
+  int64_t numel_type[kJobs];  // numel * 4 + type (0 f32, 1 bf16, 2 f16, 3 f64)
+};
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef double f64x2 __attribute__((ext_vector_type(2)));
+// 16-byte accesses at any element address (a gradient may be a slice at an odd offset)
+typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
+typedef half8 half8_u __attribute__((aligned(2)));
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+typedef f64x2 f64x2_u __attribute__((aligned(8)));
+
+template <typename T> struct Pack;
+template <> struct Pack<bf16> { typedef bf16x8_u V; static constexpr int n = 8; };
+template <> struct Pack<_Float16> { typedef half8_u V; static constexpr int n = 8; };
+template <> struct Pack<float> { typedef f32x4_u V; static constexpr int n = 4; };
+template <> struct Pack<double> { typedef f64x2_u V; static constexpr int n = 2; };
+
+template <typename T>
+__device__ __forceinline__ double sumsq_unit(const T* __restrict__ p, int64_t c0, int64_t numel) {
+  constexpr int W = Pack<T>::n, STEP = 256 * W, LOADS = kUnit / STEP, U = LOADS < 4 ? LOADS : 4;
+  double acc = 0.0;
+  if (c0 + kUnit <= numel) {
+    for (int l = 0; l < LOADS; l += U) {
+      typename Pack<T>::V v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        v[u] = *reinterpret_cast<const typename Pack<T>::V*>(p + c0 + (l + u) * STEP + threadIdx.x * W);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          const double d = (double)v[u][j];
+          acc = fma(d, d, acc);
+        }
+    }
+  } else {
+    for (int64_t i = c0 + threadIdx.x; i < numel; i += 256) {
+      const double d = (double)p[i];
+      acc = fma(d, d, acc);
+    }
+  }
+  return acc;
+}
+
+// The coefficient is used in fp32 (2^-24 relative; fp64 gradients take it whole) and each product rounded to T
+template <typename T>
+__device__ __forceinline__ void scale_unit(T* __restrict__ p, int64_t c0, int64_t numel, double coef) {
+  constexpr int W = Pack<T>::n, STEP = 256 * W, LOADS = kUnit / STEP, U = LOADS < 4 ? LOADS : 4;
+  const float cf = (float)coef;
+  auto mul = [&](T x) -> T {
+    if constexpr (sizeof(T) == 8) return x * coef;
+    else return (T)((float)x * cf);
+  };
+  if (c0 + kUnit <= numel) {
+    for (int l = 0; l < LOADS; l += U) {
+      typename Pack<T>::V v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        v[u] = *reinterpret_cast<const typename Pack<T>::V*>(p + c0 + (l + u) * STEP + threadIdx.x * W);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[u][j] = mul(v[u][j]);
+        *reinterpret_cast<typename Pack<T>::V*>(p + c0 + (l + u) * STEP + threadIdx.x * W) = v[u];
+      }
+    }
+  } else {
+    for (int64_t i = c0 + threadIdx.x; i < numel; i += 256) p[i] = mul(p[i]);
+  }
+}
+
+// This workgroup's run of units, tensor by tensor: f(pointer, type, first element, numel)
+template <typename F>
+__device__ __forceinline__ void walk_units(const NormJobs& jobs, F f) {
+  const int u0 = (int)((int64_t)jobs.units * blockIdx.x / gridDim.x);
+  const int u1 = (int)((int64_t)jobs.units * (blockIdx.x + 1) / gridDim.x);
+  if (u0 >= u1) return;
+  int lo = 0, hi = jobs.n - 1;  // the last tensor that starts at or before u0
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (jobs.start[mid] <= u0) lo = mid;
+    else hi = mid - 1;
+  }
+  int j = lo;
+  for (int u = u0; u < u1; ++u) {
+    while (u >= jobs.start[j + 1]) ++j;
+    const int64_t nt = jobs.numel_type[j];
+    f(jobs.p[j], (int)(nt & 3), (int64_t)(u - jobs.start[j]) * kUnit, nt >> 2);
+  }
+}
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+
+template <int NT>
+__device__ __forceinline__ double block_sum64(double v) {
+  __shared__ double red[NT / 64];
+  v = wave_sum64(v);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double s = 0.0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) s += red[w];
+  return s;
+}
+
+__global__ void __launch_bounds__(256) grad_sumsq_kernel(NormJobs jobs, double* __restrict__ part) {
+  double acc = 0.0;
+  walk_units(jobs, [&](void* p, int type, int64_t c0, int64_t numel) {
+    if (type == 1) acc += sumsq_unit((const bf16*)p, c0, numel);
+    else if (type == 0) acc += sumsq_unit((const float*)p, c0, numel);
+    else if (type == 2) acc += sumsq_unit((const _Float16*)p, c0, numel);
+    else acc += sumsq_unit((const double*)p, c0, numel);
+  });
+  acc = block_sum64<256>(acc);
+  if (threadIdx.x == 0) part[blockIdx.x] = acc;
+}
+
+// sumsq[0] = sum of the partials, norm[0] = its root in fp32
+__global__ void __launch_bounds__(1024) grad_norm_kernel(const double* __restrict__ part, int n,
+                                                         double* __restrict__ sumsq, float* __restrict__ norm) {
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) acc += part[i];
+  acc = block_sum64<1024>(acc);
+  if (threadIdx.x == 0) {
+    *sumsq = acc;
+    *norm = (float)sqrt(acc);
+  }
+}
+
+// A norm within the bound leaves every gradient as it is: the workgroups end without touching them.  A NaN norm
+// gives a NaN coefficient (not 1), an infinite one 0, as min(1, max_norm / (norm + 1e-6)) says.
+__global__ void __launch_bounds__(256) grad_clip_kernel(NormJobs jobs, const double* __restrict__ sumsq,
+                                                        double max_norm) {
+  const double coef = max_norm / (sqrt(*sumsq) + 1e-6);
+  if (coef >= 1.0) return;
+  walk_units(jobs, [&](void* p, int type, int64_t c0, int64_t numel) {
+    if (type == 1) scale_unit((bf16*)p, c0, numel, coef);
+    else if (type == 0) scale_unit((float*)p, c0, numel, coef);
+    else if (type == 2) scale_unit((_Float16*)p, c0, numel, coef);
+    else scale_unit((double*)p, c0, numel, coef);
+  });
+}
+
+// The launches' tables for `count` tensors: calls launch(jobs, workgroups) until every unit has been given out
+template <typename L>
+static hipError_t for_each_launch(void* const* p, const int64_t* numel, const int* type, int count, L launch) {
+  constexpr int64_t kMostUnits = 1 << 30;
+  int i = 0;
+  int64_t done = 0;  // elements of tensor i that earlier launches took
+  while (i < count) {
+    NormJobs jobs;
+    int64_t units = 0;
+    int n = 0;
+    while (i < count && n < kJobs && units < kMostUnits) {
+      const int64_t left = numel[i] - done, all = (left + kUnit - 1) / kUnit;
+      const int64_t take = all < kMostUnits - units ? all : kMostUnits - units;
+      if (take > 0) {
+        const int64_t elems = take == all ? left : take * kUnit;
+        const int size = type[i] == 0 ? 4 : type[i] == 3 ? 8 : 2;
+        jobs.p[n] = static_cast<char*>(p[i]) + done * size;
+        jobs.numel_type[n] = elems * 4 + type[i];
+        jobs.start[n++] = (int)units;
+        units += take;
+        done += elems;
+      }
+      if (take == all) {
+        ++i;
+        done = 0;
+      }
+    }
+    if (n == 0) break;
+    jobs.n = n;
+    jobs.units = (int)units;
+    jobs.start[n] = (int)units;
+    const hipError_t e = launch(jobs, (int)(units < kNormGrid ? units : kNormGrid));
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace dta
+
+using namespace dta;
+
+// Partial sums that dta_grad_sumsq needs room for (doubles)
+int64_t dta_grad_sumsq_parts(const int64_t* numel, int count) {
+  int64_t units = 0;
+  for (int i = 0; i < count; ++i) units += (numel[i] + kUnit - 1) / kUnit;
+  // full tables, plus the tables that a launch's limit on units cuts short (two for each cut), plus the last
+  return (count / kJobs + 2 * (units >> 30) + 1) * (units < kNormGrid ? units + 1 : kNormGrid);
+}
+
+// sumsq (1 double), norm (1 float); part: dta_grad_sumsq_parts doubles of scratch
+hipError_t dta_grad_sumsq(void* const* p, const int64_t* numel, const int* type, int count, double* part,
+                          int64_t parts, double* sumsq, float* norm, hipStream_t st) {
+  int64_t used = 0;
+  const hipError_t e = for_each_launch(p, numel, type, count, [&](const NormJobs& jobs, int grid) {
+    if (used + grid > parts) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(grad_sumsq_kernel, dim3(grid), dim3(256), 0, st, jobs, part + used);
+    used += grid;
+    return hipGetLastError();
+  });
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(1024), 0, st, part, (int)used, sumsq, norm);
+  return hipGetLastError();
+}
+
+hipError_t dta_grad_clip(void* const* p, const int64_t* numel, const int* type, int count, const double* sumsq,
+                         double max_norm, hipStream_t st) {
+  return for_each_launch(p, numel, type, count, [&](const NormJobs& jobs, int grid) {
+    hipLaunchKernelGGL(grad_clip_kernel, dim3(grid), dim3(256), 0, st, jobs, sumsq, max_norm);
+    return hipGetLastError();
+  });
+}

@@ -1,0 +1,35 @@
+// Launchers of preference.hip, called from bindings_pref.cpp.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace dta {
+struct PrefLogits {  // logits [B, S, V] of unit inner stride, targets [B, S]
+  const void* z;
+  int64_t sb, ss;
+  const int64_t* target;
+  int64_t tb, ts;
+  int64_t B, S, V, ignore;
+};
+struct PrefTokens {  // fp32 [B, S], strides in elements (0: broadcast); p null where absent
+  const float* p;
+  int64_t sb, ss;
+};
+}  // namespace dta
+
+// type: 0 f32, 1 bf16, 2 f16.  Scratch and state: part (dta_pref_parts float2), seg (B * dta_pref_segs double4 /
+// double2), rows (B * S float4), weight (B floats).
+int dta_pref_fits(int64_t N, int64_t V);
+int64_t dta_pref_parts(int64_t N, int64_t V);
+int64_t dta_pref_segs(int64_t S);
+hipError_t dta_pref_logprobs(const dta::PrefLogits&, int type, double temperature, void* part, float* logp, void* rows,
+                             hipStream_t);
+hipError_t dta_pref_policy(const dta::PrefLogits&, int type, double temperature, const dta::PrefTokens& old_logp,
+                           const dta::PrefTokens& ref_logp, const dta::PrefTokens& adv, double clip, double clip_high,
+                           double kl_coef, int by_sequence, double scale, void* part, double* seg, float* loss,
+                           float* stats, float* logp, void* rows, float* weight, hipStream_t);
+hipError_t dta_pref_pairs(const dta::PrefLogits&, int type, const float* ref, int64_t ref_stride, double beta,
+                          double smoothing, int average, double scale, void* part, double* seg, float* loss,
+                          float* logp, float* margin, void* rows, float* weight, hipStream_t);
+hipError_t dta_pref_grad(const dta::PrefLogits&, int type, double temperature, const void* rows, const float* weight,
+                         const dta::PrefTokens& gout, void* dz, hipStream_t);

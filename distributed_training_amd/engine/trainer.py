@@ -259,7 +259,9 @@ class Trainer:
                 if hasattr(self.model, "clip_grad_norm_"):  # native engines: global norm over the flat (sharded) grads
                     self.model.clip_grad_norm_(self.config.grad_clip)
                 else:
-                    torch.nn.utils.clip_grad_norm_(self.model.parameters(), self.config.grad_clip)
+                    from ..ops.optim import clip_grad_norm_
+
+                    clip_grad_norm_(self.model.parameters(), self.config.grad_clip)
         with prof.range_("optimizer"):
             self.optimizer.step()
         return loss

@@ -12,7 +12,7 @@ Semantics follow torch.optim exactly (tested against it), so the reference's
 """
 from __future__ import annotations
 
-from typing import Any, Dict, List, Optional
+from typing import Any, Dict, Iterable, List, Optional, Tuple, Union
 
 import torch
 
@@ -28,6 +28,102 @@ def cast_into(src: torch.Tensor, dst: torch.Tensor) -> None:
 
 def _grad32(fg_grad: torch.Tensor) -> torch.Tensor:
     return fg_grad if fg_grad.dtype == torch.float32 else fg_grad.float()
+
+
+def _fills_memory(t: torch.Tensor) -> bool:
+    """Whether the elements lie in one stretch of memory without gaps or overlaps, in any order of dimensions."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _by_device(tensors: Iterable[torch.Tensor]) -> Dict[torch.device, List[torch.Tensor]]:
+    """The tensors by device; sparse and non-floating ones are refused."""
+    found: Dict[torch.device, List[torch.Tensor]] = {}
+    for t in tensors:
+        if t.layout != torch.strided or not t.dtype.is_floating_point or t.element_size() == 1:
+            raise TypeError(f"gradient norm: dense float64, float32, bfloat16 or float16 tensors (got {t.dtype}, "
+                            f"{t.layout})")
+        found.setdefault(t.device, []).append(t.detach())
+    return found
+
+
+def grad_sumsq(tensors: Iterable[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(sum of squares, its root)`` over all elements of all tensors: a 0-dim fp64 and a 0-dim fp32 tensor on the
+    first tensor's device, with no host sync.  GPU tensors are read once by ``csrc/grad_norm.hip`` (squares summed in
+    64 bits, the same bits every call)."""
+    first: Optional[torch.Tensor] = None
+    norm: Optional[torch.Tensor] = None
+    for device, ts in _by_device(tensors).items():
+        if device.type == "cuda":
+            sq, root = native().grad_sumsq([t if _fills_memory(t) else t.contiguous() for t in ts])
+        else:
+            sq = torch.stack([t.double().square().sum() for t in ts]).sum()
+            root = sq.sqrt().float()
+        if first is None:
+            first, norm = sq, root
+        else:
+            first = first + sq.to(first.device)
+            norm = first.sqrt().float()
+    if first is None or norm is None:
+        first, norm = torch.zeros((), dtype=torch.float64), torch.zeros(())
+    return first, norm
+
+
+def grad_clip_(tensors: Iterable[torch.Tensor], sumsq: torch.Tensor, max_norm: float) -> None:
+    """Every tensor times ``min(1, max_norm / (sqrt(sumsq) + 1e-6))`` in place; ``sumsq``: the 0-dim fp64 tensor of
+    :func:`grad_sumsq`, summed over ranks where the gradients are sharded.  Within the bound nothing is touched."""
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative (got {max_norm})")
+    for device, ts in _by_device(tensors).items():
+        if device.type != "cuda":
+            coef = (float(max_norm) / (sumsq.to(device).sqrt() + 1e-6)).clamp(max=1.0)
+            for t in ts:
+                t.mul_(coef.to(t.dtype) if t.dtype == torch.float64 else coef.float())
+            continue
+        flat = [t if _fills_memory(t) else t.contiguous() for t in ts]
+        native().grad_clip_(flat, sumsq.to(device), float(max_norm))
+        for t, f in zip(ts, flat):
+            if f is not t:  # a strided view: scaled in its copy
+                t.copy_(f)
+
+
+def global_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]]) -> torch.Tensor:
+    """The 2-norm over all elements of all tensors: a 0-dim fp32 tensor (0 where there are none).  Any mix of sizes
+    and of fp64 / fp32 / bf16 / fp16."""
+    return grad_sumsq([tensors] if isinstance(tensors, torch.Tensor) else tensors)[1]
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Scale the parameters' gradients in place so that their global 2-norm is at most ``max_norm``, and return the
+    norm before (a 0-dim fp32 tensor).  As ``torch.nn.utils.clip_grad_norm_`` with its 2-norm: the coefficient is
+    ``min(1, max_norm / (norm + 1e-6))``, a NaN norm makes every gradient NaN; parameters without a gradient are
+    skipped.  On the GPU the norm is one pass over every gradient and the scaling another, left out on the device where the
+    norm is within the bound: no host sync unless ``error_if_nonfinite`` asks for one.
+
+    Gradients held by a DDP / FSDP engine: call the engine's own ``clip_grad_norm_``, which also sums over shards."""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    seen: Dict[int, torch.Tensor] = {}
+    for p in params:  # (a parameter listed twice is clipped once)
+        if p.grad is not None:
+            seen.setdefault(id(p), p.grad)
+    grads = list(seen.values())
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative (got {max_norm})")
+    if not grads:
+        return torch.zeros(())
+    sumsq, norm = grad_sumsq(grads)
+    if error_if_nonfinite and not bool(torch.isfinite(norm)):
+        raise RuntimeError(f"the global gradient norm is {float(norm)}, so the gradients cannot be clipped")
+    grad_clip_(grads, sumsq, max_norm)
+    return norm
 
 
 def _split_params(group_params: Any) -> Any:

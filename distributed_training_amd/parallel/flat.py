@@ -210,15 +210,12 @@ def clip_flat_grad_norm_(fg: FlatParamGroup, max_norm: float, comm: Any = None, 
     does not change the norm.  Returns the total norm (0-dim tensor)."""
     if not fg.prepare_grads_for_step():
         return torch.zeros((), device=fg.grad.device)
-    g = fg.grad
-    if g.is_cuda and g.dtype == torch.float32:
-        from ..ops import native
+    from ..ops.optim import grad_clip_, grad_sumsq
 
-        sq = torch.zeros(1, dtype=torch.float32, device=g.device)
-        native().flat_sumsq(g, sq, -1)
-    else:
-        sq = g.float().pow(2).sum().reshape(1)
+    g = fg.grad
+    sq64, norm = grad_sumsq([g])
     if sharded and comm is not None and comm.world_size > 1:
+        sq = sq64.float().reshape(1)
         dev = getattr(comm, "device", None)
         if dev is not None and sq.device != torch.device(dev):  # host-resident shards, device communicator
             sq_d = sq.to(dev)
@@ -226,9 +223,8 @@ def clip_flat_grad_norm_(fg: FlatParamGroup, max_norm: float, comm: Any = None, 
             sq = sq_d.to(sq.device)
         else:
             comm.all_reduce(sq, op="sum")
-    norm = sq.sqrt()
-    coef = (float(max_norm) / (norm + 1e-6)).clamp(max=1.0)
-    g.mul_(coef.to(g.dtype))
+        sq64, norm = sq.double(), sq.sqrt()
+    grad_clip_([g], sq64, max_norm)
     return norm.reshape(())
 
 

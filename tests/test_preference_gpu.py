@@ -1,0 +1,406 @@
+"""gfx950 kernels of ops/preference.py against 64-bit forms: sizes from one token, every type, rows at any address and
+stride, positions that do not count, extreme logits, streams and captured graphs."""
+import math
+
+import pytest
+import torch
+
+from distributed_training_amd.ops import preference
+from tests import preference_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _case(B, S, V, dtype, seed=0, spread=2.0):
+    g = torch.Generator().manual_seed(seed)
+    z = (torch.randn(B, S, V, generator=g) * spread).to(dtype).to(DEV)
+    target = torch.randint(V, (B, S), generator=g).to(DEV)
+    lp, _ = oracle.logprobs64(z.double(), target)
+    old = (lp.cpu() - torch.randn(B, S, generator=g).mul(8).round() / 32 - 1 / 64).float().to(DEV)
+    ref = (lp.cpu() + torch.randn(B, S, generator=g).mul(0.3)).float().to(DEV)
+    adv = torch.randn(B, S, generator=g).to(DEV)
+    if S > 2:
+        target[0, : S // 3] = -100
+    if B > 2:
+        target[2] = -100  # a sequence without tokens
+    return z, target, old, ref, adv
+
+
+def _grad_near(got, want, p, k, k_err, e, dtype):
+    """|got - want|: one rounding to the type, the probability's relative error ``e`` (oracle.stat_error) times its
+    coefficient, and the coefficient's own error ``k_err`` (fp32 products: 4 u; the slope's dependence on lp: given)."""
+    assert got.dtype == dtype and got.shape == want.shape
+    k, k_err = k.abs().unsqueeze(-1), k_err.unsqueeze(-1)
+    onehot_minus_p = (want / torch.where(k > 0, k, torch.ones_like(k))).abs()
+    tol = want.abs() * oracle.half_step(dtype) * 1.01 + k * p * e + (k_err + k * 4 * 2.0 ** -24) * onehot_minus_p * 1.01
+    off = (got.double() - want).abs() - (tol + oracle.smallest(dtype) * 1.01 + 2.0 ** -149)
+    assert (off <= 0).all(), f"off by {float(off.max())} beyond the tolerance at {int(off.argmax())}"
+
+
+SHAPES = [(1, 1, 1), (1, 1, 2), (2, 1, 7), (1, 3, 8), (2, 5, 9), (4, 3, 63), (3, 7, 257), (2, 4, 1003), (2, 3, 2048),
+          (2, 2, 2049), (1, 2, 8191), (2, 2, 8193), (2, 5, 50257), (1, 3, 128256), (2, 300, 33), (1, 1025, 520),
+          (2, 700, 4099)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,S,V", SHAPES)
+@pytest.mark.parametrize("temperature", [1.0, 0.6])
+def test_token_logprobs(B, S, V, dtype, temperature):
+    z, target, *_ = _case(B, S, V, dtype, seed=B * S + V)
+    w = torch.randn(B, S, generator=torch.Generator().manual_seed(1)).to(DEV)
+    z.requires_grad_()
+    lp = preference.token_logprobs(z, target, temperature=temperature)
+    (grad,) = torch.autograd.grad(lp, z, w)
+    z64 = z.detach().double().requires_grad_()
+    want, live = oracle.logprobs64(z64, target, temperature=temperature)
+    (gwant,) = torch.autograd.grad(want, z64, w.double())
+    e = oracle.stat_error(z64.detach(), temperature)
+    want = want.detach()
+    assert ((lp.detach().double() - want).abs() <= e + want.abs() * 2.0 ** -24).all()
+    assert (lp[~live] == 0).all() and (grad[~live] == 0).all()
+    k = w.double() / temperature * live
+    _grad_near(grad, gwant, torch.softmax(z64.detach() / temperature, -1), k, torch.zeros_like(k), e, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,S,V", [(1, 1, 1), (2, 5, 9), (4, 3, 63), (3, 7, 257), (2, 4, 1003), (4, 2, 8193), (2, 5, 50257),
+                                   (4, 2, 128256), (3, 300, 33), (2, 700, 4099)])
+@pytest.mark.parametrize("kl,high,reduction,scale", [(0.0, None, "token", 1.0), (0.1, 0.28, "sequence", 0.25)])
+def test_policy_loss(B, S, V, dtype, kl, high, reduction, scale):
+    z, target, old, ref, adv = _case(B, S, V, dtype, seed=B + S + V)
+    per_sequence = reduction == "sequence"
+    A = adv[:, 0] if per_sequence else adv
+    kw = dict(clip_high=high, kl_coef=kl, reduction=reduction, scale=scale)
+    z.requires_grad_()
+    out = preference.policy_loss(z, target, old, A, ref, **kw)
+    (grad,) = torch.autograd.grad(out.loss, z)
+    z64 = z.detach().double().requires_grad_()
+    loss, lp, mean_kl, clipped = oracle.policy64(z64, target, old, A, ref, **kw)
+    lp64 = lp.detach()
+    (gwant,) = torch.autograd.grad(loss, z64)
+    live = (target != -100).double()
+    e = oracle.stat_error(z64.detach())
+    A64 = (A.unsqueeze(1) if per_sequence else A).double().expand(B, S)
+    ratio, d = torch.exp(lp64 - old.double()), torch.where(live > 0, ref.double() - lp64, torch.zeros_like(lp64))
+    n = live.sum().clamp(min=1)
+    weight = live / n if reduction == "token" else live / live.sum(1, keepdim=True).clamp(min=1) / B
+    # d/dlp of a token's term is at most r |A| + kl |1 - exp(d)|, of its slope r |A| + kl exp(d)
+    bend = (ratio * A64.abs() + kl * d.exp()) * weight * scale
+    steep = (ratio * A64.abs() + kl * torch.expm1(d).abs()) * weight * scale
+    assert abs(float(out.loss.detach()) - float(loss.detach())) <= float((steep * e).sum()) * 1.01 + abs(float(loss.detach())) * 2.0 ** -24
+    assert ((out.logp.double() - lp64).abs() <= e + lp64.abs() * 2.0 ** -24).all()
+    kl_tol = float(((torch.expm1(d).abs() + e) * live * e).sum() / n) * 1.01 + abs(float(mean_kl)) * 2.0 ** -24
+    assert abs(float(out.kl) - float(mean_kl)) <= kl_tol
+    assert abs(float(out.clip_fraction) - float(clipped)) <= 2.0 ** -24
+    # the token's coefficient as autograd has it: the target's gradient is k (1 - p)
+    stopped = ((A64 > 0) & (ratio > 1 + (0.2 if high is None else high))) | ((A64 < 0) & (ratio < 0.8))
+    k = (torch.where(stopped, 0.0, -ratio * A64) - kl * torch.expm1(d)) * weight * scale
+    _grad_near(grad, gwant, torch.softmax(z64.detach(), -1), torch.where(live > 0, k, 0.0), bend * e, e, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,S,V", [(2, 1, 1), (2, 5, 9), (4, 3, 63), (6, 7, 257), (4, 2, 8193), (4, 5, 50257), (2, 3, 128256),
+                                   (4, 300, 33), (2, 700, 4099)])
+@pytest.mark.parametrize("smoothing,average,use_ref", [(0.0, False, True), (0.1, True, False)])
+def test_preference_loss(B, S, V, dtype, smoothing, average, use_ref):
+    z, target, *_ = _case(B, S, V, dtype, seed=B + S + V)
+    L64 = oracle.pairs64(z.double(), target, None, average=average)[1]
+    g = torch.Generator().manual_seed(3)
+    ref = (L64.cpu() + torch.randn(B, generator=g)).float().to(DEV) if use_ref else None
+    kw = dict(beta=0.7, label_smoothing=smoothing, average=average, scale=1.5)
+    z.requires_grad_()
+    out = preference.preference_loss(z, target, ref, **kw)
+    (grad,) = torch.autograd.grad(out.loss, z)
+    z64 = z.detach().double().requires_grad_()
+    loss, L, h = oracle.pairs64(z64, target, ref, **kw)
+    (gwant,) = torch.autograd.grad(loss, z64)
+    live = (target != -100).double()
+    L, h, loss = L.detach(), h.detach(), loss.detach()
+    share = live / live.sum(1, keepdim=True).clamp(min=1) if average else live
+    e = oracle.stat_error(z64.detach())
+    eL = (share * e).sum(1)
+    P = B // 2
+    eh = 0.7 * (eL[:P] + eL[P:])
+    u = 2.0 ** -24
+    assert ((out.logp.double() - L).abs() <= eL + L.abs() * u).all()
+    assert ((out.margin.double() - h).abs() <= eh + h.abs() * u).all()
+    assert abs(float(out.loss.detach()) - float(loss)) <= 1.5 * float(eh.mean()) * 1.01 + abs(float(loss)) * u
+    slope = 1.5 * 0.7 / P * (torch.sigmoid(h) - (1 - smoothing))
+    bend = 1.5 * 0.7 / P * 0.25 * eh * 1.01
+    k = torch.cat([slope, -slope]).unsqueeze(1) * share
+    _grad_near(grad, gwant, torch.softmax(z64.detach(), -1), k, torch.cat([bend, bend]).unsqueeze(1) * share, e, dtype)
+
+
+def _all_three(z, target, old, ref, adv, **kw):
+    """Losses, statistics and gradients of the three operators on one set of inputs."""
+    z = z.detach().requires_grad_()
+    a = preference.token_logprobs(z, target, **kw)
+    b = preference.policy_loss(z, target, old, adv, ref, kl_coef=0.1, **kw)
+    got = [a.detach(), b.loss.detach(), b.logp, b.kl, b.clip_fraction]
+    got += [torch.autograd.grad(a, z, torch.ones_like(a))[0], torch.autograd.grad(b.loss, z)[0]]
+    if z.dim() == 3 and z.shape[0] % 2 == 0:
+        c = preference.preference_loss(z, target)
+        got += [c.loss.detach(), c.logp, c.margin, torch.autograd.grad(c.loss, z)[0]]
+    return got
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [1003, 1008])
+def test_layouts(V, dtype):
+    """Rows of a padded vocabulary, every second sequence, shifted tokens, a buffer at an odd address, a transposed
+    vocabulary, [N, V] logits, broadcast and transposed per-token arrays: the same bits as the contiguous call."""
+    B, S = 4, 6
+    z, target, old, ref, adv = _case(B, S, V, dtype)
+    want = _all_three(z, target, old, ref, adv)
+    padded = torch.full((B, S, V + 13), float("nan"), device=DEV, dtype=dtype)
+    padded[..., 5:V + 5] = z
+    odd = torch.empty(B * S * V + 3, device=DEV, dtype=dtype)[3:].view(B, S, V)
+    odd.copy_(z)
+    spaced = torch.full((2 * B, S + 1, V), float("nan"), device=DEV, dtype=dtype)
+    spaced[::2, 1:] = z
+    turned = z.transpose(1, 2).contiguous().transpose(1, 2)
+    ttarget = target.t().contiguous().t()
+    told = torch.stack([old, old], -1)[..., 1]
+    for other in (padded[..., 5:V + 5], odd, spaced[::2, 1:], turned):
+        for x, y in zip(_all_three(other, ttarget, told, ref.t().contiguous().t(), adv), want):
+            assert torch.equal(x, y)
+    flat = _all_three(z.view(B * S, V), target.view(-1), old.view(-1), ref.view(-1), adv.view(-1))
+    for x, y in zip(flat, want):
+        assert torch.equal(x.reshape(-1), y.reshape(-1))
+    row_adv = adv[:, :1]
+    x = preference.policy_loss(z, target, old, row_adv.expand(B, S))
+    y = preference.policy_loss(z, target, old, row_adv[:, 0])
+    assert all(torch.equal(a, b) for a, b in zip(x, y))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [9, 2100, 50304])
+def test_extreme_logits(V, dtype):
+    """Rows with masked (-inf, lowest) entries, of nothing but the lowest value, of nothing but -inf, with a NaN or +inf:
+    what log_softmax says of each; a target that is masked has log-probability -inf."""
+    low = torch.finfo(dtype).min
+    z = torch.randn(1, 7, V, generator=torch.Generator().manual_seed(0)).to(dtype).to(DEV)
+    target = torch.full((1, 7), V - 1, device=DEV)
+    z[0, 0, : V // 2] = float("-inf")
+    z[0, 1, : V // 2] = low
+    z[0, 2] = low
+    z[0, 3] = float("-inf")
+    z[0, 4, 1] = float("nan")
+    z[0, 5, 2] = float("inf")
+    z[0, 6, V - 1] = float("-inf")
+    z.requires_grad_()
+    lp = preference.token_logprobs(z, target)
+    (grad,) = torch.autograd.grad(lp.sum(), z)
+    z64 = z.detach().double().requires_grad_()
+    want = torch.log_softmax(z64, -1)[..., V - 1]
+    (gwant,) = torch.autograd.grad(want.sum(), z64)
+    # (unit-normal rows: the exponents reach under 12 nats, as stat_error counts them for the ordinary row 6)
+    e = oracle.stat_error(z64.detach()[:, 6:, :-1]) + 2.0 ** -24 * 64
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isnan(lp), torch.isnan(want)) and torch.equal(torch.isinf(lp), torch.isinf(want))
+    assert ((lp.double() - want).abs()[fine] <= e + want.abs()[fine] * 2.0 ** -24).all()
+    for row in (0, 1, 2, 6):
+        off = (grad[0, row].double() - gwant[0, row]).abs()
+        assert (off <= gwant[0, row].abs() * (oracle.half_step(dtype) * 1.01 + 4 * 2.0 ** -24) + e + oracle.smallest(dtype) * 1.01).all()
+    for row in (3, 4, 5):
+        assert torch.isnan(grad[0, row]).all() == torch.isnan(gwant[0, row]).all()
+
+
+def test_positions_that_do_not_count():
+    """Not read: NaN there reaches nothing; targets outside the vocabulary are positions that do not count."""
+    z, target, old, ref, adv = _case(4, 9, 777, torch.bfloat16)
+    dead = target == -100
+    assert dead.any()
+    want = _all_three(z, target, old, ref, adv)
+    target[0, 0], target[0, 1], target[0, 2] = 777, -7, 2 ** 40
+    for t in (z, old, ref, adv):
+        t[dead] = float("nan")
+    for x, y in zip(_all_three(z, target, old, ref, adv), want):
+        assert torch.equal(x, y)
+    moved = torch.where(target == -100, 5, target)  # another ignore_index
+    live_five = (target == 5) & ~dead
+    assert not live_five.any()
+    for x, y in zip(_all_three(z, moved, old, ref, adv, ignore_index=5)[:7], want[:7]):
+        assert torch.equal(x, y)
+
+
+def test_nothing_counts_and_nothing_there():
+    z = torch.randn(2, 3, 50, device=DEV, requires_grad=True)
+    target = torch.full((2, 3), -100, device=DEV)
+    nan = torch.full((2, 3), float("nan"), device=DEV)
+    for reduction in ("token", "sequence"):
+        out = preference.policy_loss(z, target, nan, nan, nan, kl_coef=0.1, reduction=reduction)
+        assert out.loss.item() == 0 and out.kl.item() == 0 and out.clip_fraction.item() == 0
+        assert (torch.autograd.grad(out.loss, z)[0] == 0).all()
+    out = preference.preference_loss(z, target)
+    assert abs(out.loss.item() - math.log(2)) < 1e-6 and (out.margin == 0).all()
+    assert (torch.autograd.grad(out.loss, z)[0] == 0).all()
+    for shape in ((2, 0, 50), (0, 50)):
+        z = torch.randn(shape, device=DEV, requires_grad=True)
+        target = torch.zeros(shape[:-1], dtype=torch.long, device=DEV)
+        none = torch.zeros(shape[:-1], device=DEV)
+        lp = preference.token_logprobs(z, target)
+        out = preference.policy_loss(z, target, none, none)
+        assert lp.shape == target.shape and out.loss.item() == 0
+        assert torch.autograd.grad(out.loss + lp.sum(), z)[0].shape == z.shape
+
+
+def test_offsets_past_32_bits():
+    """Logits of more than 2^31 elements: the last sequence's values and gradients are those of its own call."""
+    B, S, V = 4, 4200, 128256
+    assert B * S * V > 2 ** 31
+    z = torch.zeros(B, S, V, device=DEV, dtype=torch.bfloat16)
+    z[-1].normal_(0, 2, generator=torch.Generator(device=DEV).manual_seed(0))
+    target = torch.full((B, S), -100, device=DEV)
+    target[-1] = torch.randint(V, (S,), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    old = torch.full((B, S), -11.5, device=DEV)
+    adv = torch.linspace(-1, 1, S, device=DEV).expand(B, S)
+    z.requires_grad_()
+    out = preference.policy_loss(z, target, old, adv)
+    (grad,) = torch.autograd.grad(out.loss, z)
+    tail = z.detach()[-1:].clone().requires_grad_()
+    want = preference.policy_loss(tail, target[-1:], old[-1:], adv[-1:])
+    (gwant,) = torch.autograd.grad(want.loss, tail)
+    assert torch.equal(out.loss, want.loss) and torch.equal(out.logp[-1:], want.logp)
+    assert torch.equal(grad[-1:], gwant)
+    assert not grad[0].any() and not grad[2].any()
+
+
+def test_backward_twice_scaled_and_other_uses():
+    """A retained graph's second backward, a scaled loss, a leaf that accumulates: each as the formula says."""
+    z, target, old, ref, adv = _case(4, 6, 1003, torch.float32)
+    z.requires_grad_()
+    for make in (lambda: preference.policy_loss(z, target, old, adv, ref, kl_coef=0.1).loss,
+                 lambda: preference.preference_loss(z, target).loss,
+                 lambda: preference.token_logprobs(z, target).mean()):
+        (g1,) = torch.autograd.grad(make(), z)
+        loss = make()
+        (a,) = torch.autograd.grad(loss, z, retain_graph=True)
+        a.zero_()  # what backward returned belongs to the caller
+        (b,) = torch.autograd.grad(loss, z, retain_graph=True)
+        (c,) = torch.autograd.grad(loss * 4.0, z)
+        assert torch.equal(b, g1) and torch.equal(c, 4.0 * g1)
+        z.grad = None
+        make().backward()
+        (make() * 0.5).backward()
+        torch.testing.assert_close(z.grad, 1.5 * g1, rtol=2.0 ** -22, atol=2.0 ** -149)
+        z.grad = None
+    scaled = preference.policy_loss(z, target, old, adv, ref, kl_coef=0.1, scale=0.25)
+    full = preference.policy_loss(z, target, old, adv, ref, kl_coef=0.1)
+    assert torch.equal(scaled.loss, 0.25 * full.loss)
+    assert torch.equal(torch.autograd.grad(scaled.loss, z)[0], 0.25 * torch.autograd.grad(full.loss, z)[0])
+    with torch.no_grad():
+        assert torch.equal(preference.policy_loss(z, target, old, adv, ref, kl_coef=0.1).loss, full.loss)
+    with pytest.raises(RuntimeError):  # no second derivatives
+        (g,) = torch.autograd.grad(preference.preference_loss(z, target).loss, z, create_graph=True)
+        g.sum().backward()
+    loss = preference.preference_loss(z.clone(), target).loss
+    y = z.clone()
+    loss = preference.policy_loss(y, target, old, adv).loss
+    y.mul_(2.0)  # the logits changed since the forward: autograd says so
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_same_bits_every_call_and_other_streams():
+    z, target, old, ref, adv = _case(4, 40, 9973, torch.bfloat16)
+    want = _all_three(z, target, old, ref, adv)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams * 2:  # two streams at once
+        with torch.cuda.stream(s):
+            got.append(_all_three(z, target, old, ref, adv))
+    torch.cuda.synchronize()
+    for other in got:
+        assert all(torch.equal(x, y) for x, y in zip(other, want))
+
+
+def test_captured_and_replayed():
+    """Forward and backward of the three operators in one graph, replayed on new inputs between eager calls."""
+    shape = (4, 12, 5003)
+    fixed = [t.clone() for t in _case(*shape, torch.bfloat16)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _all_three(*fixed)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _all_three(*fixed)
+    for seed in range(1, 5):
+        new = _case(*shape, torch.bfloat16, seed=seed)
+        want = _all_three(*new)
+        for f, n in zip(fixed, new):
+            f.copy_(n)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+        del want, new
+
+
+def test_refusals_on_the_device():
+    z, target, old, ref, adv = _case(2, 3, 50, torch.float32)
+    with pytest.raises(TypeError, match="GPU logits"):
+        preference.token_logprobs(z.double(), target)
+    with pytest.raises(ValueError, match="logits on"):
+        preference.token_logprobs(z, target.cpu())
+    with pytest.raises(ValueError, match="logits on"):
+        preference.policy_loss(z, target, old.cpu(), adv)
+    with pytest.raises(TypeError, match="float32"):
+        preference.policy_loss(z, target, old, adv.double())
+    with pytest.raises(ValueError, match="logits on"):
+        preference.preference_loss(z, target, torch.zeros(2))
+
+
+def test_a_preference_step_end_to_end():
+    """A reference model scores, the policy under the DDP engine is trained on pairs and on rewards, gradients are
+    clipped, the optimizer steps: the run of operators as a training program has them, its gradients against the same
+    run with the losses in 64 bits."""
+    from distributed_training_amd.models.gpt2 import GPT2, GPT2Config
+    from distributed_training_amd.ops.optim import FusedAdamW
+    from distributed_training_amd.parallel.comm import RcclComm
+    from distributed_training_amd.parallel.ddp import DistributedDataParallel
+
+    torch.manual_seed(0)
+    dev = torch.device(DEV, 0)
+    model = GPT2(GPT2Config(n_layer=2, n_head=2, n_embd=128, vocab_size=1000, block_size=64)).to(dev)
+    w = DistributedDataParallel(model, comm=RcclComm(0, 1, dev), device=dev, param_dtype=torch.bfloat16)
+    opt = FusedAdamW(w.parameters(), lr=1e-3)
+    idx = torch.randint(1000, (4, 64), device=DEV)
+    target = torch.roll(idx, -1, 1)
+    target[:, :8] = -100
+    target[:, -1] = -100
+    adv = torch.tensor([1.0, -0.5, 0.8, -1.2], device=DEV)
+    with torch.no_grad():
+        ref_tok = preference.token_logprobs(w(idx), target)
+
+    def loss_of(logits, exact):
+        if exact:
+            z = logits.double()
+            return (oracle.policy64(z, target, ref_tok + 0.1, adv, ref_tok, kl_coef=0.05)[0]
+                    + oracle.pairs64(z, target, ref_tok.sum(1))[0]).float()
+        return (preference.policy_loss(logits, target, ref_tok + 0.1, adv, ref_tok, kl_coef=0.05).loss
+                + preference.preference_loss(logits, target, ref_tok.sum(1)).loss)
+
+    for step in range(2):
+        grads = []
+        for exact in (True, False):
+            w.zero_grad(set_to_none=True)
+            loss_of(w(idx), exact).backward()
+            torch.cuda.synchronize()
+            grads.append([p.grad.double().clone() for p in w.parameters()])
+        for a, b in zip(*grads):
+            # the logit gradients of the two losses are rounded to bf16 before their sum is (half a step each, 2^-9 of a
+            # term), and what follows rounds at each of the 2 layers' 8 products and norms: a few of those steps in norm
+            assert (a - b).norm() <= 16 * 2.0 ** -9 * a.norm() + 1e-6
+        want = math.sqrt(sum(float(g.square().sum()) for g in grads[1]))
+        norm = w.clip_grad_norm_(0.1)
+        assert want > 0.1 and abs(float(norm) - want) <= 2.0 ** -23 * want
+        for p, g in zip(w.parameters(), grads[1]):
+            g = g * (0.1 / (want + 1e-6))
+            assert ((p.grad.double() - g).abs() <= g.abs() * (oracle.half_step(p.grad.dtype) + 2.0 ** -22)).all()
+        opt.step()
+    assert all(torch.isfinite(p).all() for p in w.parameters())
