@@ -2,12 +2,14 @@
 // gradient norm over many tensors (csrc/grad_norm.hip), registered into the same _C module by dta_register_pref.
 //
 // Every entry point checks device / dtype / shape / strides on the host before enqueueing, runs on its tensors'
-// device whatever the current one is, and takes its scratch from the caching allocator on the stream it uses.
+// device whatever the current one is, and takes its scratch from the caching allocator on the stream it uses.  The
+// losses are autograd functions here rather than in Python: a small batch's pass is all host time.
 #include <torch/extension.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <unordered_set>
 #include <vector>
 
 #include "preference.h"
@@ -20,6 +22,8 @@ hipError_t dta_grad_clip(void* const*, const int64_t*, const int*, int, const do
 namespace {
 
 using torch::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 using OptTensor = c10::optional<torch::Tensor>;
 
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
@@ -27,6 +31,14 @@ bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
 void ok(hipError_t e, const char* what) { TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e)); }
 
 hipStream_t stream_on(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+// 0 while nothing is being captured on the stream
+unsigned long long capture_of(hipStream_t st) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  ok(hipStreamGetCaptureInfo(st, &status, &id), "hipStreamGetCaptureInfo");
+  return status == hipStreamCaptureStatusNone ? 0 : id;
+}
 
 int float_type(const Tensor& t) {
   switch (t.scalar_type()) {
@@ -38,25 +50,27 @@ int float_type(const Tensor& t) {
   }
 }
 
-// ------------------------------------------------------------------ preference losses
+// ------------------------------------------------------------------ arguments
 // logits [B, S, V] or [N, V] (one sequence of N tokens), unit inner stride; target int64 of the leading shape
 dta::PrefLogits logits_arg(const Tensor& z, const Tensor& target, int64_t ignore, int* type) {
-  TORCH_CHECK(z.is_cuda() && target.is_cuda() && z.device() == target.device(),
-              "logits and target must be on the same GPU");
-  TORCH_CHECK(z.dim() == 2 || z.dim() == 3, "logits must be [N, V] or [B, S, V]");
-  TORCH_CHECK(target.dim() == z.dim() - 1 && target.sizes() == z.sizes().slice(0, z.dim() - 1),
-              "target must have the logits' shape without the vocabulary");
-  TORCH_CHECK_TYPE(target.scalar_type() == torch::kInt64, "target must be int64");
+  TORCH_CHECK_TYPE(z.defined() && target.defined(), "logits and target must be tensors");
+  TORCH_CHECK_VALUE(z.is_cuda(), "logits must be on a GPU (got ", z.device(), ")");
+  TORCH_CHECK_VALUE(z.dim() == 2 || z.dim() == 3, "logits must be [N, V] or [B, S, V] (got ", z.sizes(), ")");
+  TORCH_CHECK_VALUE(target.sizes() == z.sizes().slice(0, z.dim() - 1), "target must be ",
+                    z.sizes().slice(0, z.dim() - 1), " (got ", target.sizes(), ")");
+  TORCH_CHECK_VALUE(target.device() == z.device(), "target is on ", target.device(), ", logits on ", z.device());
+  TORCH_CHECK_TYPE(target.scalar_type() == torch::kInt64, "target must be int64 (got ", target.scalar_type(), ")");
   *type = float_type(z);
-  TORCH_CHECK_TYPE(*type >= 0 && *type <= 2, "logits must be float32, bfloat16 or float16");
+  TORCH_CHECK_TYPE(*type >= 0 && *type <= 2, "GPU logits must be bfloat16, float16 or float32 (got ",
+                   z.scalar_type(), ")");
   const bool flat = z.dim() == 2;
   dta::PrefLogits l{};
   l.V = z.size(-1);
   l.S = z.size(-2);
   l.B = flat ? 1 : z.size(0);
-  TORCH_CHECK(l.V >= 1, "logits must have a vocabulary");
-  TORCH_CHECK(l.V == 1 || z.stride(-1) == 1, "logits must have unit inner stride");
-  TORCH_CHECK(dta_pref_fits(l.B * l.S, l.V), "logits: too many rows for one launch");
+  TORCH_CHECK_VALUE(l.V >= 1, "logits must have a vocabulary");
+  TORCH_CHECK_VALUE(l.V == 1 || z.stride(-1) == 1, "logits must have unit inner stride");
+  TORCH_CHECK_VALUE(dta_pref_fits(l.B * l.S, l.V), "logits: too many rows for one launch");
   l.z = z.data_ptr();
   l.ss = z.stride(-2);
   l.sb = flat ? 0 : z.stride(0);
@@ -68,120 +82,232 @@ dta::PrefLogits logits_arg(const Tensor& z, const Tensor& target, int64_t ignore
 }
 
 // A per-token fp32 array; per_sequence: [B] stands for each token of its sequence
-dta::PrefTokens tokens_arg(const OptTensor& t, const Tensor& target, const char* name, bool per_sequence = false) {
-  if (!has(t)) return {nullptr, 0, 0};
-  TORCH_CHECK(t->device() == target.device(), name, " must be on the logits' GPU");
-  TORCH_CHECK_TYPE(t->scalar_type() == torch::kFloat32, name, " must be float32");
+dta::PrefTokens tokens_arg(const Tensor& t, const Tensor& target, const char* name, bool per_sequence = false) {
+  TORCH_CHECK_TYPE(t.defined(), name, " must be a tensor");
   const bool flat = target.dim() == 1;
-  if (per_sequence && !flat && t->dim() == 1) {
-    TORCH_CHECK(t->size(0) == target.size(0), name, " must be [B] or [B, S]");
-    return {t->data_ptr<float>(), t->stride(0), 0};
+  const bool one_each = per_sequence && !flat && t.dim() == 1 && t.size(0) == target.size(0);
+  TORCH_CHECK_VALUE(one_each || t.sizes() == target.sizes(), name, " must be ", target.sizes(),
+                    per_sequence && !flat ? " or one a sequence" : "", " (got ", t.sizes(), ")");
+  TORCH_CHECK_VALUE(t.device() == target.device(), name, " is on ", t.device(), ", logits on ", target.device());
+  TORCH_CHECK_TYPE(t.scalar_type() == torch::kFloat32, name, " must be float32 (got ", t.scalar_type(), ")");
+  if (one_each) return {t.data_ptr<float>(), t.stride(0), 0};
+  return {t.data_ptr<float>(), flat ? 0 : t.stride(0), t.stride(-1)};
+}
+
+Tensor unit_stride(const Tensor& z) {
+  return z.defined() && z.dim() >= 2 && z.size(-1) != 1 && z.stride(-1) != 1 ? z.contiguous() : z;
+}
+
+bool wants_grad(const Tensor& z) { return torch::GradMode::is_enabled() && z.requires_grad(); }
+
+// One allocation of scratch and state: sections of `bytes`, each 256-byte aligned
+struct Arena {
+  int64_t size = 0;
+  Tensor t;
+  int64_t add(int64_t bytes) {
+    const int64_t at = size;
+    size += (bytes + 255) / 256 * 256;
+    return at;
   }
-  TORCH_CHECK(t->sizes() == target.sizes(), name, per_sequence ? " must be [B] or [B, S]" : " must have target's shape");
-  return {t->data_ptr<float>(), flat ? 0 : t->stride(0), t->stride(-1)};
-}
+  void make(const Tensor& like) { t = torch::empty({size > 0 ? size : 1}, like.options().dtype(torch::kUInt8)); }
+  char* at(int64_t off) const { return static_cast<char*>(t.data_ptr()) + off; }
+};
 
-void temperature_arg(double t) {
-  TORCH_CHECK_VALUE(std::isfinite(t) && t > 0.0, "temperature must be positive and finite");
-}
+// ------------------------------------------------------------------ gradient of the logits
+// state: [rows: 16 N bytes, rounded up to 256][sequence weights]
+int64_t weight_at(int64_t N) { return (16 * N + 255) / 256 * 256; }
 
-// -> log-probabilities of target's shape, row state
-std::vector<Tensor> pref_logprobs(Tensor logits, Tensor target, int64_t ignore_index, double temperature) {
+void logits_grad(const Tensor& z, const Tensor& target, const Tensor& state, bool weighted, const Tensor& g,
+                 int64_t ignore, double temperature, bool unless_one, const Tensor& dz) {
+  // (a second derivative would need more than this formula: refused rather than silently wrong)
+  TORCH_CHECK(!(torch::GradMode::is_enabled() && g.requires_grad()),
+              "the preference losses can be differentiated once: no create_graph through them");
   int type;
-  const auto l = logits_arg(logits, target, ignore_index, &type);
-  temperature_arg(temperature);
-  const at::DeviceGuard guard(logits.device());
-  const auto f32 = logits.options().dtype(torch::kFloat32);
-  const int64_t N = l.B * l.S;
-  Tensor logp = torch::empty(target.sizes(), f32), rows = torch::empty({N, 4}, f32);
-  Tensor part = torch::empty({dta_pref_parts(N, l.V), 2}, f32);
-  ok(dta_pref_logprobs(l, type, temperature, part.data_ptr(), logp.data_ptr<float>(), rows.data_ptr(),
-                       stream_on(logits)),
-     "token_logprobs");
-  return {logp, rows};
+  const auto l = logits_arg(z, target, ignore, &type);
+  const Tensor gf = g.scalar_type() == torch::kFloat32 ? g : g.to(torch::kFloat32);
+  const dta::PrefTokens gout = gf.dim() == 0 ? dta::PrefTokens{gf.data_ptr<float>(), 0, 0}
+                                             : tokens_arg(gf, target, "gradient");
+  TORCH_CHECK(gf.device() == z.device(), "gradient is on ", gf.device(), ", logits on ", z.device());
+  char* s = static_cast<char*>(state.data_ptr());
+  ok(dta_pref_grad(l, type, temperature, s, weighted ? reinterpret_cast<float*>(s + weight_at(l.B * l.S)) : nullptr,
+                   gout, unless_one, dz.data_ptr(), stream_on(z)),
+     "logits gradient");
 }
 
-// -> loss, {kl, clip fraction}, log-probabilities, row state, sequence weights
-std::vector<Tensor> pref_policy(Tensor logits, Tensor target, Tensor old_logp, Tensor advantages, OptTensor ref_logp,
-                                double clip, double clip_high, double kl_coef, bool by_sequence, int64_t ignore_index,
-                                double temperature, double scale) {
-  int type;
-  const auto l = logits_arg(logits, target, ignore_index, &type);
-  temperature_arg(temperature);
-  const auto old_a = tokens_arg(old_logp, target, "old_logp"), ref_a = tokens_arg(ref_logp, target, "ref_logp");
-  const auto adv_a = tokens_arg(advantages, target, "advantages", true);
-  const at::DeviceGuard guard(logits.device());
-  const auto f32 = logits.options().dtype(torch::kFloat32);
-  const int64_t N = l.B * l.S;
-  Tensor loss = torch::empty({}, f32), stats = torch::empty({2}, f32);
-  Tensor logp = torch::empty(target.sizes(), f32), rows = torch::empty({N, 4}, f32);
-  Tensor weight = torch::empty({l.B}, f32), part = torch::empty({dta_pref_parts(N, l.V), 2}, f32);
-  Tensor seg = torch::empty({l.B * dta_pref_segs(l.S), 4}, f32.dtype(torch::kFloat64));
-  ok(dta_pref_policy(l, type, temperature, old_a, ref_a, adv_a, clip, clip_high, kl_coef, by_sequence, scale,
-                     part.data_ptr(), seg.data_ptr<double>(), loss.data_ptr<float>(), stats.data_ptr<float>(),
-                     logp.data_ptr<float>(), rows.data_ptr(), weight.data_ptr<float>(), stream_on(logits)),
-     "policy_loss");
-  return {loss, stats, logp, rows, weight};
-}
-
-// -> loss, sequence log-probabilities [B], margins [B / 2], row state, sequence weights
-std::vector<Tensor> pref_pairs(Tensor logits, Tensor target, OptTensor ref_logp, double beta, double smoothing,
-                               bool average, int64_t ignore_index, double scale) {
-  int type;
-  TORCH_CHECK(logits.dim() == 3, "logits must be [2 * pairs, S, V]");
-  const auto l = logits_arg(logits, target, ignore_index, &type);
-  TORCH_CHECK(l.B >= 2 && l.B % 2 == 0, "logits must hold the chosen sequences, then as many rejected ones");
-  const float* ref = nullptr;
-  int64_t ref_stride = 0;
-  if (has(ref_logp)) {
-    TORCH_CHECK(ref_logp->device() == logits.device(), "ref_logp must be on the logits' GPU");
-    TORCH_CHECK_TYPE(ref_logp->scalar_type() == torch::kFloat32, "ref_logp must be float32");
-    TORCH_CHECK(ref_logp->dim() == 1 && ref_logp->size(0) == l.B, "ref_logp must be [2 * pairs]");
-    ref = ref_logp->data_ptr<float>();
-    ref_stride = ref_logp->stride(0);
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& z, const Tensor& target, int64_t ignore,
+                        double temperature) {
+    int type;
+    const auto l = logits_arg(z, target, ignore, &type);
+    const at::DeviceGuard guard(z.device());
+    const int64_t N = l.B * l.S;
+    Arena a;
+    const int64_t rows = a.add(16 * N), part = a.add(16 * dta_pref_parts(N, l.V));
+    a.make(z);
+    Tensor logp = torch::empty(target.sizes(), z.options().dtype(torch::kFloat32));
+    ok(dta_pref_logprobs(l, type, temperature, a.at(part), logp.data_ptr<float>(), a.at(rows), stream_on(z)),
+       "token_logprobs");
+    ctx->save_for_backward({z, target, a.t});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["temperature"] = temperature;
+    return logp;
   }
-  const at::DeviceGuard guard(logits.device());
-  const auto f32 = logits.options().dtype(torch::kFloat32);
-  const int64_t N = l.B * l.S;
-  Tensor loss = torch::empty({}, f32), logp = torch::empty({l.B}, f32), margin = torch::empty({l.B / 2}, f32);
-  Tensor rows = torch::empty({N, 4}, f32), weight = torch::empty({l.B}, f32);
-  Tensor part = torch::empty({dta_pref_parts(N, l.V), 2}, f32);
-  Tensor seg = torch::empty({l.B * dta_pref_segs(l.S), 2}, f32.dtype(torch::kFloat64));
-  ok(dta_pref_pairs(l, type, ref, ref_stride, beta, smoothing, average, scale, part.data_ptr(), seg.data_ptr<double>(),
-                    loss.data_ptr<float>(), logp.data_ptr<float>(), margin.data_ptr<float>(), rows.data_ptr(),
-                    weight.data_ptr<float>(), stream_on(logits)),
-     "preference_loss");
-  return {loss, logp, margin, rows, weight};
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &z = saved[0], &target = saved[1];
+    const at::DeviceGuard guard(z.device());
+    Tensor dz = torch::empty(z.sizes(), z.options());
+    logits_grad(z, target, saved[2], false, grads[0], ctx->saved_data["ignore"].toInt(),
+                ctx->saved_data["temperature"].toDouble(), false, dz);
+    return {dz, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& z, const Tensor& target, const Tensor& old_logp,
+                               const Tensor& advantages, const OptTensor& ref_logp, double clip, double clip_high,
+                               double kl_coef, bool by_sequence, int64_t ignore, double temperature, double scale,
+                               bool grad) {
+    int type;
+    const auto l = logits_arg(z, target, ignore, &type);
+    dta::PrefPolicy p{};
+    p.old_logp = tokens_arg(old_logp, target, "old_logp");
+    if (has(ref_logp)) p.ref_logp = tokens_arg(*ref_logp, target, "ref_logp");
+    p.adv = tokens_arg(advantages, target, "advantages", true);
+    p.clip = clip;
+    p.clip_high = clip_high;
+    p.kl_coef = kl_coef;
+    p.scale = scale;
+    p.by_sequence = by_sequence;
+    const at::DeviceGuard guard(z.device());
+    const hipStream_t st = stream_on(z);
+    const int64_t N = l.B * l.S;
+    const bool fused = grad && dta_pref_policy_fused(type, N, l.V);
+    Arena a;
+    const int64_t rows = a.add(16 * N), weight = a.add(4 * l.B);
+    const int64_t part = a.add(fused ? 32 * N + 8 : 16 * dta_pref_parts(N, l.V));
+    const int64_t seg = a.add(fused ? 0 : 32 * dta_pref_segs(l.B, l.S, l.V));
+    a.make(z);
+    const auto f32 = z.options().dtype(torch::kFloat32);
+    Tensor loss = torch::empty({}, f32), stats = torch::empty({2}, f32), logp = torch::empty(target.sizes(), f32);
+    if (fused) {
+      Tensor dz = torch::empty(z.sizes(), z.options());
+      ok(dta_pref_policy_grad(l, type, temperature, p, reinterpret_cast<double*>(a.at(part)), loss.data_ptr<float>(),
+                              stats.data_ptr<float>(), logp.data_ptr<float>(), a.at(rows),
+                              reinterpret_cast<float*>(a.at(weight)), dz.data_ptr(), st),
+         "policy_loss");
+      ctx->saved_data["dz"] = dz;
+      ctx->saved_data["capture"] = (int64_t)capture_of(st);
+    } else {
+      ok(dta_pref_policy(l, type, temperature, p, a.at(part), reinterpret_cast<double*>(a.at(seg)),
+                         loss.data_ptr<float>(), stats.data_ptr<float>(), logp.data_ptr<float>(), a.at(rows),
+                         reinterpret_cast<float*>(a.at(weight)), st),
+         "policy_loss");
+    }
+    ctx->save_for_backward({z, target, a.t});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["temperature"] = temperature;
+    ctx->set_materialize_grads(false);
+    Tensor kl = stats[0], clipped = stats[1];
+    ctx->mark_non_differentiable({logp, kl, clipped});
+    return {loss, logp, kl, clipped};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list none(13);
+    if (!grads[0].defined()) return none;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &z = saved[0], &target = saved[1];
+    const at::DeviceGuard guard(z.device());
+    // The gradient that the forward wrote for a loss gradient of 1 goes to the first backward, which rewrites it where
+    // another came; a second backward over a retained graph writes its own.  So does one that is captured into a graph
+    // without its forward: a replay would find what its caller has made of the buffer since.
+    Tensor dz;
+    auto& data = ctx->saved_data;
+    const auto it = data.find("dz");
+    if (it != data.end()) {
+      if (data["capture"].toInt() == (int64_t)capture_of(stream_on(z))) dz = it->second.toTensor();
+      data.erase("dz");
+    }
+    const bool written = dz.defined();
+    if (!written) dz = torch::empty(z.sizes(), z.options());
+    logits_grad(z, target, saved[2], true, grads[0], data["ignore"].toInt(), data["temperature"].toDouble(), written,
+                dz);
+    none[0] = dz;
+    return none;
+  }
+};
+
+struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& z, const Tensor& target, const OptTensor& ref_logp,
+                               double beta, double smoothing, bool average, int64_t ignore, double scale) {
+    int type;
+    const auto l = logits_arg(z, target, ignore, &type);
+    TORCH_CHECK_VALUE(z.dim() == 3 && l.B >= 2 && l.B % 2 == 0,
+                      "logits must be [2 P, S, V]: P chosen sequences, then as many rejected ones (got ", z.sizes(),
+                      ")");
+    const float* ref = nullptr;
+    int64_t ref_stride = 0;
+    if (has(ref_logp)) {
+      TORCH_CHECK_VALUE(ref_logp->dim() == 1 && ref_logp->size(0) == l.B, "ref_logp must be [", l.B, "] (got ",
+                        ref_logp->sizes(), ")");
+      TORCH_CHECK_VALUE(ref_logp->device() == z.device(), "ref_logp is on ", ref_logp->device(), ", logits on ",
+                        z.device());
+      TORCH_CHECK_TYPE(ref_logp->scalar_type() == torch::kFloat32, "ref_logp must be float32 (got ",
+                       ref_logp->scalar_type(), ")");
+      ref = ref_logp->data_ptr<float>();
+      ref_stride = ref_logp->stride(0);
+    }
+    const at::DeviceGuard guard(z.device());
+    const int64_t N = l.B * l.S;
+    Arena a;
+    const int64_t rows = a.add(16 * N), weight = a.add(4 * l.B), part = a.add(16 * dta_pref_parts(N, l.V));
+    const int64_t seg = a.add(16 * dta_pref_segs(l.B, l.S, l.V));
+    a.make(z);
+    const auto f32 = z.options().dtype(torch::kFloat32);
+    Tensor loss = torch::empty({}, f32), logp = torch::empty({l.B}, f32), margin = torch::empty({l.B / 2}, f32);
+    ok(dta_pref_pairs(l, type, ref, ref_stride, beta, smoothing, average, scale, a.at(part),
+                      reinterpret_cast<double*>(a.at(seg)), loss.data_ptr<float>(), logp.data_ptr<float>(),
+                      margin.data_ptr<float>(), a.at(rows), reinterpret_cast<float*>(a.at(weight)), stream_on(z)),
+       "preference_loss");
+    ctx->save_for_backward({z, target, a.t});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({logp, margin});
+    return {loss, logp, margin};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list none(8);
+    if (!grads[0].defined()) return none;
+    const auto saved = ctx->get_saved_variables();
+    const at::DeviceGuard guard(saved[0].device());
+    Tensor dz = torch::empty(saved[0].sizes(), saved[0].options());
+    logits_grad(saved[0], saved[1], saved[2], true, grads[0], ctx->saved_data["ignore"].toInt(), 1.0, false, dz);
+    none[0] = dz;
+    return none;
+  }
+};
+
+Tensor token_logprobs(const Tensor& logits, const Tensor& target, int64_t ignore_index, double temperature) {
+  return TokenLogprobs::apply(unit_stride(logits), target, ignore_index, temperature);
 }
 
-// gout: a scalar, or one gradient a token (target's shape)
-Tensor pref_grad(Tensor logits, Tensor target, Tensor rows, OptTensor weight, Tensor gout, int64_t ignore_index,
-                 double temperature) {
-  int type;
-  const auto l = logits_arg(logits, target, ignore_index, &type);
-  temperature_arg(temperature);
-  const int64_t N = l.B * l.S;
-  TORCH_CHECK(rows.device() == logits.device() && rows.scalar_type() == torch::kFloat32 && rows.is_contiguous() &&
-                  rows.numel() == 4 * N,
-              "row state: f32 [N, 4]");
-  const float* w = nullptr;
-  if (has(weight)) {
-    TORCH_CHECK(weight->device() == logits.device() && weight->scalar_type() == torch::kFloat32 &&
-                    weight->is_contiguous() && weight->numel() == l.B,
-                "sequence weights: f32 [B]");
-    w = weight->data_ptr<float>();
-  }
-  dta::PrefTokens g{};
-  if (gout.dim() == 0) {
-    TORCH_CHECK(gout.device() == logits.device() && gout.scalar_type() == torch::kFloat32, "gradient: f32 scalar");
-    g = {gout.data_ptr<float>(), 0, 0};
-  } else {
-    g = tokens_arg(gout, target, "gradient");
-  }
-  const at::DeviceGuard guard(logits.device());
-  Tensor dz = torch::empty(logits.sizes(), logits.options());
-  ok(dta_pref_grad(l, type, temperature, rows.data_ptr(), w, g, dz.data_ptr(), stream_on(logits)), "logits gradient");
-  return dz;
+std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& target,
+                                                       const Tensor& old_logp, const Tensor& advantages,
+                                                       const OptTensor& ref_logp, double clip, double clip_high,
+                                                       double kl_coef, bool by_sequence, int64_t ignore_index,
+                                                       double temperature, double scale) {
+  const Tensor z = unit_stride(logits);
+  const auto r = PolicyLoss::apply(z, target, old_logp, advantages, ref_logp, clip, clip_high, kl_coef, by_sequence,
+                                   ignore_index, temperature, scale, z.defined() && wants_grad(z));
+  return {r[0], r[1], r[2], r[3]};
+}
+
+std::tuple<Tensor, Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& target,
+                                                   const OptTensor& ref_logp, double beta, double smoothing,
+                                                   bool average, int64_t ignore_index, double scale) {
+  const auto r = PreferenceLoss::apply(unit_stride(logits), target, ref_logp, beta, smoothing, average, ignore_index,
+                                       scale);
+  return {r[0], r[1], r[2]};
 }
 
 // ------------------------------------------------------------------ gradient norm
@@ -189,42 +315,46 @@ struct GradList {
   std::vector<void*> p;
   std::vector<int64_t> numel;
   std::vector<int> type;
+  void add(const Tensor& t, int type_) {
+    p.push_back(t.data_ptr());
+    numel.push_back(t.numel());
+    type.push_back(type_);
+  }
 };
 
 GradList grads_arg(const std::vector<Tensor>& ts) {
   GradList g;
   TORCH_CHECK(!ts.empty(), "no tensors");
-  g.p.reserve(ts.size());
-  g.numel.reserve(ts.size());
-  g.type.reserve(ts.size());
   for (const auto& t : ts) {
     TORCH_CHECK(t.is_cuda() && t.device() == ts[0].device(), "gradients must be on one GPU");
     const int type = float_type(t);
     TORCH_CHECK_TYPE(type >= 0, "gradients must be float32, bfloat16, float16 or float64");
     TORCH_CHECK(t.is_non_overlapping_and_dense(), "gradients must be dense in memory");
-    g.p.push_back(t.data_ptr());
-    g.numel.push_back(t.numel());
-    g.type.push_back(type);
+    g.add(t, type);
   }
   return g;
 }
 
 // -> sum of squares (f64 scalar), norm (f32 scalar)
-std::vector<Tensor> grad_sumsq(std::vector<Tensor> grads) {
-  const GradList g = grads_arg(grads);
-  const at::DeviceGuard guard(grads[0].device());
-  const int n = (int)grads.size();
-  const auto f64 = torch::TensorOptions().device(grads[0].device()).dtype(torch::kFloat64);
+std::tuple<Tensor, Tensor> sumsq_of(const GradList& g, c10::Device device, hipStream_t st) {
+  const auto f64 = torch::TensorOptions().device(device).dtype(torch::kFloat64);
+  const int n = (int)g.p.size();
   const int64_t parts = dta_grad_sumsq_parts(g.numel.data(), n);
   Tensor part = torch::empty({parts}, f64), sumsq = torch::empty({}, f64);
   Tensor norm = torch::empty({}, f64.dtype(torch::kFloat32));
   ok(dta_grad_sumsq(g.p.data(), g.numel.data(), g.type.data(), n, part.data_ptr<double>(), parts,
-                    sumsq.data_ptr<double>(), norm.data_ptr<float>(), stream_on(grads[0])),
+                    sumsq.data_ptr<double>(), norm.data_ptr<float>(), st),
      "grad_sumsq");
   return {sumsq, norm};
 }
 
-void grad_clip_(std::vector<Tensor> grads, Tensor sumsq, double max_norm) {
+std::tuple<Tensor, Tensor> grad_sumsq(const std::vector<Tensor>& grads) {
+  const GradList g = grads_arg(grads);
+  const at::DeviceGuard guard(grads[0].device());
+  return sumsq_of(g, grads[0].device(), stream_on(grads[0]));
+}
+
+void grad_clip_(const std::vector<Tensor>& grads, const Tensor& sumsq, double max_norm) {
   const GradList g = grads_arg(grads);
   TORCH_CHECK(sumsq.device() == grads[0].device() && sumsq.scalar_type() == torch::kFloat64 && sumsq.numel() == 1,
               "sumsq: f64 scalar on the gradients' GPU");
@@ -232,21 +362,47 @@ void grad_clip_(std::vector<Tensor> grads, Tensor sumsq, double max_norm) {
   ok(dta_grad_clip(g.p.data(), g.numel.data(), g.type.data(), (int)grads.size(), sumsq.data_ptr<double>(), max_norm,
                    stream_on(grads[0])),
      "grad_clip");
+  for (const auto& t : grads) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// The whole of clip_grad_norm_ for parameters whose gradients all lie dense on one GPU: the norm, or None where they
+// do not (ops/optim.py then takes them one device and one layout at a time).
+OptTensor clip_params_(const std::vector<Tensor>& params, double max_norm) {
+  GradList g;
+  std::vector<Tensor> grads;
+  std::unordered_set<const void*> seen;
+  for (const auto& p : params) {
+    const Tensor& t = p.grad();
+    if (!t.defined() || !seen.insert(p.unsafeGetTensorImpl()).second) continue;  // listed twice: clipped once
+    if (t.layout() != torch::kStrided || !t.is_cuda() || (!grads.empty() && t.device() != grads[0].device()) ||
+        float_type(t) < 0 || !t.is_non_overlapping_and_dense())
+      return c10::nullopt;
+    g.add(t, float_type(t));
+    grads.push_back(t);
+  }
+  if (grads.empty()) return c10::nullopt;
+  const at::DeviceGuard guard(grads[0].device());
+  const hipStream_t st = stream_on(grads[0]);
+  const auto sn = sumsq_of(g, grads[0].device(), st);
+  ok(dta_grad_clip(g.p.data(), g.numel.data(), g.type.data(), (int)g.p.size(), std::get<0>(sn).data_ptr<double>(),
+                   max_norm, st),
+     "grad_clip");
+  for (const auto& t : grads) t.unsafeGetTensorImpl()->bump_version();
+  return std::get<1>(sn);
 }
 
 }  // namespace
 
 void dta_register_pref(pybind11::module_& m) {
   namespace py = pybind11;
-  m.def("pref_logprobs", &pref_logprobs, py::arg("logits"), py::arg("target"), py::arg("ignore_index"),
+  m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("target"), py::arg("ignore_index"),
         py::arg("temperature"));
-  m.def("pref_policy", &pref_policy, py::arg("logits"), py::arg("target"), py::arg("old_logp"), py::arg("advantages"),
+  m.def("policy_loss", &policy_loss, py::arg("logits"), py::arg("target"), py::arg("old_logp"), py::arg("advantages"),
         py::arg("ref_logp"), py::arg("clip"), py::arg("clip_high"), py::arg("kl_coef"), py::arg("by_sequence"),
         py::arg("ignore_index"), py::arg("temperature"), py::arg("scale"));
-  m.def("pref_pairs", &pref_pairs, py::arg("logits"), py::arg("target"), py::arg("ref_logp"), py::arg("beta"),
-        py::arg("smoothing"), py::arg("average"), py::arg("ignore_index"), py::arg("scale"));
-  m.def("pref_grad", &pref_grad, py::arg("logits"), py::arg("target"), py::arg("rows"), py::arg("weight"),
-        py::arg("gout"), py::arg("ignore_index"), py::arg("temperature"));
+  m.def("preference_loss", &preference_loss, py::arg("logits"), py::arg("target"), py::arg("ref_logp"),
+        py::arg("beta"), py::arg("smoothing"), py::arg("average"), py::arg("ignore_index"), py::arg("scale"));
   m.def("grad_sumsq", &grad_sumsq, py::arg("grads"));
   m.def("grad_clip_", &grad_clip_, py::arg("grads"), py::arg("sumsq"), py::arg("max_norm"));
+  m.def("clip_params_", &clip_params_, py::arg("params"), py::arg("max_norm"));
 }

@@ -15,21 +15,30 @@ struct PrefTokens {  // fp32 [B, S], strides in elements (0: broadcast); p null 
   const float* p;
   int64_t sb, ss;
 };
+struct PrefPolicy {
+  PrefTokens old_logp, ref_logp, adv;
+  double clip, clip_high, kl_coef, scale;
+  int by_sequence;
+};
 }  // namespace dta
 
-// type: 0 f32, 1 bf16, 2 f16.  Scratch and state: part (dta_pref_parts float2), seg (B * dta_pref_segs double4 /
-// double2), rows (B * S float4), weight (B floats).
+// type: 0 f32, 1 bf16, 2 f16.  Scratch and state: part (dta_pref_parts x 16 bytes), seg (dta_pref_segs double4 / double2),
+// terms (B * S double4 and one double), rows (B * S float4), weight (B floats).
 int dta_pref_fits(int64_t N, int64_t V);
 int64_t dta_pref_parts(int64_t N, int64_t V);
-int64_t dta_pref_segs(int64_t S);
+int64_t dta_pref_segs(int64_t B, int64_t S, int64_t V);
 hipError_t dta_pref_logprobs(const dta::PrefLogits&, int type, double temperature, void* part, float* logp, void* rows,
                              hipStream_t);
-hipError_t dta_pref_policy(const dta::PrefLogits&, int type, double temperature, const dta::PrefTokens& old_logp,
-                           const dta::PrefTokens& ref_logp, const dta::PrefTokens& adv, double clip, double clip_high,
-                           double kl_coef, int by_sequence, double scale, void* part, double* seg, float* loss,
-                           float* stats, float* logp, void* rows, float* weight, hipStream_t);
+hipError_t dta_pref_policy(const dta::PrefLogits&, int type, double temperature, const dta::PrefPolicy&, void* part,
+                           double* seg, float* loss, float* stats, float* logp, void* rows, float* weight, hipStream_t);
+// the loss with the gradient of the logits for a loss gradient of 1, in one pass; for sizes that dta_pref_policy_fused takes
+int dta_pref_policy_fused(int type, int64_t N, int64_t V);
+hipError_t dta_pref_policy_grad(const dta::PrefLogits&, int type, double temperature, const dta::PrefPolicy&,
+                                double* terms, float* loss, float* stats, float* logp, void* rows, float* weight,
+                                void* dz, hipStream_t);
 hipError_t dta_pref_pairs(const dta::PrefLogits&, int type, const float* ref, int64_t ref_stride, double beta,
                           double smoothing, int average, double scale, void* part, double* seg, float* loss,
                           float* logp, float* margin, void* rows, float* weight, hipStream_t);
+// unless_one: dz holds the gradient for gout = 1 already; rewritten only where the (scalar) gout is another
 hipError_t dta_pref_grad(const dta::PrefLogits&, int type, double temperature, const void* rows, const float* weight,
-                         const dta::PrefTokens& gout, void* dz, hipStream_t);
+                         const dta::PrefTokens& gout, int unless_one, void* dz, hipStream_t);

@@ -109,14 +109,18 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     norm is within the bound: no host sync unless ``error_if_nonfinite`` asks for one.
 
     Gradients held by a DDP / FSDP engine: call the engine's own ``clip_grad_norm_``, which also sums over shards."""
-    params = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative (got {max_norm})")
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    if not error_if_nonfinite and params and params[0].is_cuda:
+        norm = native().clip_params_(params, float(max_norm))  # one call for gradients that lie dense on one GPU
+        if norm is not None:
+            return norm
     seen: Dict[int, torch.Tensor] = {}
     for p in params:  # (a parameter listed twice is clipped once)
         if p.grad is not None:
             seen.setdefault(id(p), p.grad)
     grads = list(seen.values())
-    if not max_norm >= 0.0:
-        raise ValueError(f"max_norm must not be negative (got {max_norm})")
     if not grads:
         return torch.zeros(())
     sumsq, norm = grad_sumsq(grads)

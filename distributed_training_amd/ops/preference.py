@@ -7,18 +7,17 @@ a position does not count (prompts, padding).  Positions that do not count -- a 
 ``[0, V)`` -- have log-probability 0 and a zero gradient, whatever their logits hold.
 
 GPU tensors take the HIP kernels of ``csrc/preference.hip`` (bf16, fp16 or fp32 logits; rows of any stride and
-alignment, any vocabulary).  CPU tensors take the same math in PyTorch, which is also the tests' reference.  Per-token
-inputs are fp32; statistics over the vocabulary are fp32, per-token terms and sums fp64.
+alignment, any vocabulary) through the autograd functions of ``csrc/bindings_pref.cpp``, which check their tensors.
+CPU tensors take the same math in PyTorch.  Per-token inputs are fp32; statistics over the vocabulary are fp32,
+per-token terms and sums fp64.  Each loss can be differentiated once.
 """
 from __future__ import annotations
 
 import math
-from typing import Any, NamedTuple, Optional, Tuple
+from typing import NamedTuple, Optional
 
 import torch
 import torch.nn.functional as F
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import native
 
@@ -56,8 +55,6 @@ def _check(logits: torch.Tensor, target: torch.Tensor) -> None:
         raise ValueError(f"target is on {target.device}, logits on {logits.device}")
     if not logits.dtype.is_floating_point:
         raise TypeError(f"logits must be floating point (got {logits.dtype})")
-    if logits.is_cuda and logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise TypeError(f"GPU logits must be bfloat16, float16 or float32 (got {logits.dtype})")
 
 
 def _check_tokens(t: Optional[torch.Tensor], target: torch.Tensor, name: str, per_sequence: bool = False) -> None:
@@ -66,7 +63,7 @@ def _check_tokens(t: Optional[torch.Tensor], target: torch.Tensor, name: str, pe
     shapes = [target.shape] + ([target.shape[:1]] if per_sequence and target.dim() == 2 else [])
     if t.shape not in shapes:
         raise ValueError(f"{name} must be {' or '.join(str(tuple(s)) for s in shapes)} (got {tuple(t.shape)})")
-    if t.dtype != torch.float32 and not (t.dtype == torch.float64 and not t.is_cuda):
+    if t.dtype not in (torch.float32, torch.float64):
         raise TypeError(f"{name} must be float32 (got {t.dtype})")
     if t.device != target.device:
         raise ValueError(f"{name} is on {t.device}, logits on {target.device}")
@@ -84,10 +81,6 @@ def _not_negative(x: float, name: str) -> float:
     return float(x)
 
 
-def _unit_stride(logits: torch.Tensor) -> torch.Tensor:
-    return logits if logits.shape[-1] == 1 or logits.stride(-1) == 1 else logits.contiguous()
-
-
 # ------------------------------------------------------------------ token log-probabilities
 def _live(logits: torch.Tensor, target: torch.Tensor, ignore_index: int) -> torch.Tensor:
     return (target != ignore_index) & (target >= 0) & (target < logits.shape[-1])
@@ -103,31 +96,14 @@ def token_logprobs_reference(logits: torch.Tensor, target: torch.Tensor, ignore_
     return lp.masked_fill(~live, 0.0)
 
 
-class _TokenLogprobs(Function):
-    @staticmethod
-    def forward(ctx: Any, logits: torch.Tensor, target: torch.Tensor, ignore_index: int,
-                temperature: float) -> torch.Tensor:
-        logp, rows = native().pref_logprobs(logits, target, ignore_index, temperature)
-        ctx.save_for_backward(logits, target, rows)
-        ctx.cfg = (ignore_index, temperature)
-        return logp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, g: torch.Tensor) -> Tuple[Optional[torch.Tensor], ...]:
-        logits, target, rows = ctx.saved_tensors
-        ignore_index, temperature = ctx.cfg
-        return native().pref_grad(logits, target, rows, None, g, ignore_index, temperature), None, None, None
-
-
 def token_logprobs(logits: torch.Tensor, target: torch.Tensor, ignore_index: int = -100,
                    temperature: float = 1.0) -> torch.Tensor:
     """``log softmax(logits / temperature)`` at each position's target: fp32, of ``target``'s shape, 0 where a position
     does not count.  What a rollout stores as ``old_logp`` and a frozen model gives as ``ref_logp``; differentiable."""
-    _check(logits, target)
     temperature = _positive(temperature, "temperature")
     if logits.is_cuda:
-        return _TokenLogprobs.apply(_unit_stride(logits), target, int(ignore_index), temperature)
+        return native().token_logprobs(logits, target, ignore_index, temperature)
+    _check(logits, target)
     return token_logprobs_reference(logits, target, ignore_index, temperature)
 
 
@@ -164,30 +140,6 @@ def policy_loss_reference(logits: torch.Tensor, target: torch.Tensor, old_logp: 
                       (clipped.sum() / tokens).to(logp.dtype))
 
 
-class _PolicyLoss(Function):
-    @staticmethod
-    def forward(ctx: Any, logits: torch.Tensor, target: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
-                ref_logp: Optional[torch.Tensor], clip: float, clip_high: float, kl_coef: float, by_sequence: bool,
-                ignore_index: int, temperature: float, scale: float) -> Tuple[torch.Tensor, ...]:
-        loss, stats, logp, rows, weight = native().pref_policy(logits, target, old_logp, advantages, ref_logp, clip,
-                                                               clip_high, kl_coef, by_sequence, ignore_index,
-                                                               temperature, scale)
-        ctx.save_for_backward(logits, target, rows, weight)
-        ctx.cfg = (ignore_index, temperature)
-        ctx.mark_non_differentiable(stats, logp)
-        ctx.set_materialize_grads(False)
-        return loss, stats, logp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, g: Optional[torch.Tensor], *_: Any) -> Tuple[Optional[torch.Tensor], ...]:
-        if g is None:
-            return (None,) * 12
-        logits, target, rows, weight = ctx.saved_tensors
-        ignore_index, temperature = ctx.cfg
-        return (native().pref_grad(logits, target, rows, weight, g, ignore_index, temperature),) + (None,) * 11
-
-
 def policy_loss(logits: torch.Tensor, target: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
                 ref_logp: Optional[torch.Tensor] = None, clip: float = 0.2, clip_high: Optional[float] = None,
                 kl_coef: float = 0.0, reduction: str = "token", ignore_index: int = -100, temperature: float = 1.0,
@@ -202,10 +154,6 @@ def policy_loss(logits: torch.Tensor, target: torch.Tensor, old_logp: torch.Tens
     differs from ``clip``.  ``reduction``: ``"token"`` -- the mean over all tokens that count; ``"sequence"`` -- the mean over the
     B sequences of each one's token mean (an empty sequence adds 0).  ``scale`` multiplies the loss: with gradient
     accumulation pass 1 / steps here rather than dividing the result.  No token counting: the loss is 0."""
-    _check(logits, target)
-    for t, name in ((old_logp, "old_logp"), (ref_logp, "ref_logp")):
-        _check_tokens(t, target, name)
-    _check_tokens(advantages, target, "advantages", per_sequence=True)
     clip, kl_coef = _not_negative(clip, "clip"), _not_negative(kl_coef, "kl_coef")
     clip_high = clip if clip_high is None else _not_negative(clip_high, "clip_high")
     temperature = _positive(temperature, "temperature")
@@ -213,15 +161,17 @@ def policy_loss(logits: torch.Tensor, target: torch.Tensor, old_logp: torch.Tens
         raise ValueError(f"scale must be finite (got {scale})")
     if reduction not in ("token", "sequence"):
         raise ValueError(f"reduction must be 'token' or 'sequence' (got {reduction!r})")
-    if reduction == "sequence" and logits.dim() != 3:
+    if reduction == "sequence" and logits.dim() == 2:
         raise ValueError("reduction='sequence' needs logits [B, S, V]")
     if kl_coef and ref_logp is None:
         raise ValueError("kl_coef needs ref_logp")
     if logits.is_cuda:
-        loss, stats, logp = _PolicyLoss.apply(_unit_stride(logits), target, old_logp.detach(), advantages.detach(),
-                                              None if ref_logp is None else ref_logp.detach(), clip, clip_high, kl_coef,
-                                              reduction == "sequence", int(ignore_index), temperature, float(scale))
-        return PolicyLoss(loss, logp, stats[0], stats[1])
+        return PolicyLoss(*native().policy_loss(logits, target, old_logp, advantages, ref_logp, clip, clip_high, kl_coef,
+                                                reduction == "sequence", ignore_index, temperature, scale))
+    _check(logits, target)
+    for t, name in ((old_logp, "old_logp"), (ref_logp, "ref_logp")):
+        _check_tokens(t, target, name)
+    _check_tokens(advantages, target, "advantages", per_sequence=True)
     return policy_loss_reference(logits, target, old_logp.detach(), advantages.detach(),
                                  None if ref_logp is None else ref_logp.detach(), clip, clip_high, kl_coef, reduction,
                                  ignore_index, temperature, scale)
@@ -244,27 +194,6 @@ def preference_loss_reference(logits: torch.Tensor, target: torch.Tensor, ref_lo
     return PreferenceLoss(loss.to(lp.dtype), total.detach().to(lp.dtype), h.detach().to(lp.dtype))
 
 
-class _PreferenceLoss(Function):
-    @staticmethod
-    def forward(ctx: Any, logits: torch.Tensor, target: torch.Tensor, ref_logp: Optional[torch.Tensor], beta: float,
-                label_smoothing: float, average: bool, ignore_index: int, scale: float) -> Tuple[torch.Tensor, ...]:
-        loss, logp, margin, rows, weight = native().pref_pairs(logits, target, ref_logp, beta, label_smoothing, average,
-                                                               ignore_index, scale)
-        ctx.save_for_backward(logits, target, rows, weight)
-        ctx.ignore_index = ignore_index
-        ctx.mark_non_differentiable(logp, margin)
-        ctx.set_materialize_grads(False)
-        return loss, logp, margin
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, g: Optional[torch.Tensor], *_: Any) -> Tuple[Optional[torch.Tensor], ...]:
-        if g is None:
-            return (None,) * 8
-        logits, target, rows, weight = ctx.saved_tensors
-        return (native().pref_grad(logits, target, rows, weight, g, ctx.ignore_index, 1.0),) + (None,) * 7
-
-
 def preference_loss(logits: torch.Tensor, target: torch.Tensor, ref_logp: Optional[torch.Tensor] = None,
                     beta: float = 0.1, label_smoothing: float = 0.0, average: bool = False, ignore_index: int = -100,
                     scale: float = 1.0) -> PreferenceLoss:
@@ -277,6 +206,14 @@ def preference_loss(logits: torch.Tensor, target: torch.Tensor, ref_logp: Option
     ``logits`` ``[2 P, S, V]``: the P chosen sequences, then the P rejected ones in the same order (one forward over both).
     ``ref_logp`` ``[2 P]`` fp32: the frozen model's ``L`` of the same sequences, formed the same way (absent: 0).
     ``scale`` as in :func:`policy_loss`.  A sequence without tokens that count has ``L = 0``."""
+    beta = _positive(beta, "beta")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"label_smoothing must be in [0, 1] (got {label_smoothing})")
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite (got {scale})")
+    if logits.is_cuda:
+        return PreferenceLoss(*native().preference_loss(logits, target, ref_logp, beta, label_smoothing, average,
+                                                        ignore_index, scale))
     _check(logits, target)
     if logits.dim() != 3 or logits.shape[0] < 2 or logits.shape[0] % 2:
         raise ValueError("logits must be [2 P, S, V]: P chosen sequences, then as many rejected ones "
@@ -286,12 +223,4 @@ def preference_loss(logits: torch.Tensor, target: torch.Tensor, ref_logp: Option
             raise ValueError(f"ref_logp must be {tuple(logits.shape[:1])} (got {tuple(ref_logp.shape)})")
         _check_tokens(ref_logp, target[:, 0] if target.shape[1] else ref_logp, "ref_logp")
         ref_logp = ref_logp.detach()
-    beta = _positive(beta, "beta")
-    if not 0.0 <= label_smoothing <= 1.0:
-        raise ValueError(f"label_smoothing must be in [0, 1] (got {label_smoothing})")
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite (got {scale})")
-    if logits.is_cuda:
-        return PreferenceLoss(*_PreferenceLoss.apply(_unit_stride(logits), target, ref_logp, beta, float(label_smoothing),
-                                                     bool(average), int(ignore_index), float(scale)))
     return preference_loss_reference(logits, target, ref_logp, beta, label_smoothing, average, ignore_index, scale)

@@ -163,12 +163,14 @@ def test_native_entry_points_refuse_host_tensors():
     C = native()
     z, target, old, ref, adv = _inputs(dtype=torch.float32)
     old, adv = old.float(), adv.float()
-    with pytest.raises(RuntimeError, match="same GPU"):
-        C.pref_logprobs(z, target, -100, 1.0)
-    with pytest.raises(RuntimeError, match="same GPU"):
-        C.pref_policy(z, target, old, adv, None, 0.2, 0.2, 0.0, False, -100, 1.0, 1.0)
-    with pytest.raises(RuntimeError, match="same GPU"):
-        C.pref_pairs(z, target, None, 0.1, 0.0, False, -100, 1.0)
+    with pytest.raises(ValueError, match="on a GPU"):
+        C.token_logprobs(z, target, -100, 1.0)
+    with pytest.raises(ValueError, match="on a GPU"):
+        C.policy_loss(z, target, old, adv, None, 0.2, 0.2, 0.0, False, -100, 1.0, 1.0)
+    with pytest.raises(ValueError, match="on a GPU"):
+        C.preference_loss(z, target, None, 0.1, 0.0, False, -100, 1.0)
+    with pytest.raises(TypeError):
+        C.token_logprobs(z, None, -100, 1.0)
     with pytest.raises(RuntimeError, match="one GPU"):
         C.grad_sumsq([z])
     with pytest.raises(RuntimeError, match="no tensors"):

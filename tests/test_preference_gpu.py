@@ -46,7 +46,7 @@ SHAPES = [(1, 1, 1), (1, 1, 2), (2, 1, 7), (1, 3, 8), (2, 5, 9), (4, 3, 63), (3,
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B,S,V", SHAPES)
-@pytest.mark.parametrize("temperature", [1.0, 0.6])
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
 def test_token_logprobs(B, S, V, dtype, temperature):
     z, target, *_ = _case(B, S, V, dtype, seed=B * S + V)
     w = torch.randn(B, S, generator=torch.Generator().manual_seed(1)).to(DEV)
@@ -66,7 +66,9 @@ def test_token_logprobs(B, S, V, dtype, temperature):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B,S,V", [(1, 1, 1), (2, 5, 9), (4, 3, 63), (3, 7, 257), (2, 4, 1003), (4, 2, 8193), (2, 5, 50257),
-                                   (4, 2, 128256), (3, 300, 33), (2, 700, 4099)])
+                                   (4, 2, 128256), (3, 300, 33), (2, 700, 4099), (1, 512, 1), (3, 257, 8192), (2, 300, 16383),
+                                   (1, 520, 24577), (1, 515, 32767), (2, 257, 50257), (1, 512, 53248), (1, 514, 65535),
+                                   (1, 513, 70001), (4, 130, 128256)])
 @pytest.mark.parametrize("kl,high,reduction,scale", [(0.0, None, "token", 1.0), (0.1, 0.28, "sequence", 0.25)])
 def test_policy_loss(B, S, V, dtype, kl, high, reduction, scale):
     z, target, old, ref, adv = _case(B, S, V, dtype, seed=B + S + V)
@@ -147,11 +149,11 @@ def _all_three(z, target, old, ref, adv, **kw):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("V", [1003, 1008])
-def test_layouts(V, dtype):
+@pytest.mark.parametrize("S,V", [(6, 1003), (6, 1008), (131, 1003)])
+def test_layouts(S, V, dtype):
     """Rows of a padded vocabulary, every second sequence, shifted tokens, a buffer at an odd address, a transposed
     vocabulary, [N, V] logits, broadcast and transposed per-token arrays: the same bits as the contiguous call."""
-    B, S = 4, 6
+    B = 4
     z, target, old, ref, adv = _case(B, S, V, dtype)
     want = _all_three(z, target, old, ref, adv)
     padded = torch.full((B, S, V + 13), float("nan"), device=DEV, dtype=dtype)
@@ -177,7 +179,8 @@ def test_layouts(V, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V", [9, 2100, 50304])
-def test_extreme_logits(V, dtype):
+@pytest.mark.parametrize("temperature", [1.0, 0.7, 1.5, 1.4426950408889634])  # log2(e) / temperature rounds down, up, is 1
+def test_extreme_logits(V, dtype, temperature):
     """Rows with masked (-inf, lowest) entries, of nothing but the lowest value, of nothing but -inf, with a NaN or +inf:
     what log_softmax says of each; a target that is masked has log-probability -inf."""
     low = torch.finfo(dtype).min
@@ -191,13 +194,13 @@ def test_extreme_logits(V, dtype):
     z[0, 5, 2] = float("inf")
     z[0, 6, V - 1] = float("-inf")
     z.requires_grad_()
-    lp = preference.token_logprobs(z, target)
+    lp = preference.token_logprobs(z, target, temperature=temperature)
     (grad,) = torch.autograd.grad(lp.sum(), z)
     z64 = z.detach().double().requires_grad_()
-    want = torch.log_softmax(z64, -1)[..., V - 1]
+    want = torch.log_softmax(z64 / temperature, -1)[..., V - 1]
     (gwant,) = torch.autograd.grad(want.sum(), z64)
     # (unit-normal rows: the exponents reach under 12 nats, as stat_error counts them for the ordinary row 6)
-    e = oracle.stat_error(z64.detach()[:, 6:, :-1]) + 2.0 ** -24 * 64
+    e = oracle.stat_error(z64.detach()[:, 6:, :-1], temperature) + 2.0 ** -24 * 64
     fine = torch.isfinite(want)
     assert torch.equal(torch.isnan(lp), torch.isnan(want)) and torch.equal(torch.isinf(lp), torch.isinf(want))
     assert ((lp.double() - want).abs()[fine] <= e + want.abs()[fine] * 2.0 ** -24).all()
@@ -208,9 +211,11 @@ def test_extreme_logits(V, dtype):
         assert torch.isnan(grad[0, row]).all() == torch.isnan(gwant[0, row]).all()
 
 
-def test_positions_that_do_not_count():
+@pytest.mark.parametrize("S", [9, 200])
+def test_positions_that_do_not_count(S):
     """Not read: NaN there reaches nothing; targets outside the vocabulary are positions that do not count."""
-    z, target, old, ref, adv = _case(4, 9, 777, torch.bfloat16)
+    z, target, old, ref, adv = _case(4, S, 777, torch.bfloat16)
+    target[target == 5] = 6
     dead = target == -100
     assert dead.any()
     want = _all_three(z, target, old, ref, adv)
@@ -220,8 +225,6 @@ def test_positions_that_do_not_count():
     for x, y in zip(_all_three(z, target, old, ref, adv), want):
         assert torch.equal(x, y)
     moved = torch.where(target == -100, 5, target)  # another ignore_index
-    live_five = (target == 5) & ~dead
-    assert not live_five.any()
     for x, y in zip(_all_three(z, moved, old, ref, adv, ignore_index=5)[:7], want[:7]):
         assert torch.equal(x, y)
 
@@ -268,9 +271,10 @@ def test_offsets_past_32_bits():
     assert not grad[0].any() and not grad[2].any()
 
 
-def test_backward_twice_scaled_and_other_uses():
+@pytest.mark.parametrize("S", [6, 150])  # few rows, and enough for the policy loss's one-pass form
+def test_backward_twice_scaled_and_other_uses(S):
     """A retained graph's second backward, a scaled loss, a leaf that accumulates: each as the formula says."""
-    z, target, old, ref, adv = _case(4, 6, 1003, torch.float32)
+    z, target, old, ref, adv = _case(4, S, 1003, torch.float32)
     z.requires_grad_()
     for make in (lambda: preference.policy_loss(z, target, old, adv, ref, kl_coef=0.1).loss,
                  lambda: preference.preference_loss(z, target).loss,
@@ -304,8 +308,9 @@ def test_backward_twice_scaled_and_other_uses():
         loss.backward()
 
 
-def test_same_bits_every_call_and_other_streams():
-    z, target, old, ref, adv = _case(4, 40, 9973, torch.bfloat16)
+@pytest.mark.parametrize("S", [40, 140])
+def test_same_bits_every_call_and_other_streams(S):
+    z, target, old, ref, adv = _case(4, S, 9973, torch.bfloat16)
     want = _all_three(z, target, old, ref, adv)
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
@@ -318,9 +323,9 @@ def test_same_bits_every_call_and_other_streams():
         assert all(torch.equal(x, y) for x, y in zip(other, want))
 
 
-def test_captured_and_replayed():
+@pytest.mark.parametrize("shape", [(4, 12, 5003), (4, 130, 2003)])
+def test_captured_and_replayed(shape):
     """Forward and backward of the three operators in one graph, replayed on new inputs between eager calls."""
-    shape = (4, 12, 5003)
     fixed = [t.clone() for t in _case(*shape, torch.bfloat16)]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -404,3 +409,32 @@ def test_a_preference_step_end_to_end():
             assert ((p.grad.double() - g).abs() <= g.abs() * (oracle.half_step(p.grad.dtype) + 2.0 ** -22)).all()
         opt.step()
     assert all(torch.isfinite(p).all() for p in w.parameters())
+
+
+@pytest.mark.parametrize("V", [2100, 50304])
+def test_extreme_logits_in_one_pass(V):
+    """The policy loss's one-pass form on rows with -inf and lowest entries agrees with the form for few rows, and a row that
+    is NaN by the definition makes its own gradient NaN and no other's."""
+    z = torch.randn(1, 600, V, generator=torch.Generator().manual_seed(0)).bfloat16().to(DEV)
+    target = torch.full((1, 600), V - 1, device=DEV)
+    z[0, 0, : V // 2] = float("-inf")
+    z[0, 1, : V // 2] = torch.finfo(torch.bfloat16).min
+    z[0, 2] = torch.finfo(torch.bfloat16).min
+    old, adv = torch.full((1, 600), -8.0, device=DEV), torch.ones(1, 600, device=DEV)
+    few = slice(0, 40)
+
+    def grads(z, n, scale):
+        z = z.detach().requires_grad_()
+        out = preference.policy_loss(z, target[:, :n], old[:, :n], adv[:, :n], clip_high=1e9, scale=scale)
+        return out.logp, torch.autograd.grad(out.loss, z)[0]
+
+    lp, g = grads(z, 600, 600.0)
+    lp_few, g_few = grads(z[:, few], 40, 40.0)
+    e = oracle.stat_error(z[:, 3:].double())
+    assert torch.isfinite(g).all()
+    assert ((lp[:, few] - lp_few).abs() <= 2 * e + lp_few.abs() * 2.0 ** -23).all()
+    assert ((g[:, few].double() - g_few.double()).abs() <= g_few.double().abs() * 2.0 ** -7 + 4 * e * math.exp(8.0)).all()
+    z[0, 3], z[0, 4, 7], z[0, 5, 9] = float("-inf"), float("nan"), float("inf")
+    lp, g = grads(z, 600, 600.0)
+    assert torch.isnan(lp[0, 3:6]).all() and torch.isnan(g[0, 3:6]).all()
+    assert torch.isfinite(lp[0, 6:]).all() and torch.isfinite(g[0, 6:]).all() and torch.isfinite(g[0, :3]).all()
