@@ -261,7 +261,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     const int64_t N = l.B * l.S;
     Arena a;
     const int64_t rows = a.add(16 * N), weight = a.add(4 * l.B), part = a.add(16 * dta_pref_parts(N, l.V));
-    const int64_t seg = a.add(16 * dta_pref_segs(l.B, l.S, l.V));
+    const int64_t seg = a.add(16 * (dta_pref_segs(l.B, l.S, l.V) + l.B));
     a.make(z);
     const auto f32 = z.options().dtype(torch::kFloat32);
     Tensor loss = torch::empty({}, f32), logp = torch::empty({l.B}, f32), margin = torch::empty({l.B / 2}, f32);

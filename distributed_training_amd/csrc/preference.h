@@ -22,8 +22,8 @@ struct PrefPolicy {
 };
 }  // namespace dta
 
-// type: 0 f32, 1 bf16, 2 f16.  Scratch and state: part (dta_pref_parts x 16 bytes), seg (dta_pref_segs double4 / double2),
-// terms (B * S double4 and one double), rows (B * S float4), weight (B floats).
+// type: 0 f32, 1 bf16, 2 f16.  Scratch and state: part (dta_pref_parts x 16 bytes), seg (dta_pref_segs double4; pairs:
+// dta_pref_segs + B double2), terms (B * S double4 and one double), rows (B * S float4), weight (B floats).
 int dta_pref_fits(int64_t N, int64_t V);
 int64_t dta_pref_parts(int64_t N, int64_t V);
 int64_t dta_pref_segs(int64_t B, int64_t S, int64_t V);

@@ -34,72 +34,39 @@ template <typename V>
 __device__ __forceinline__ V load_nt(const void* p) { return __builtin_nontemporal_load(static_cast<const V*>(p)); }
 template <typename V>
 __device__ __forceinline__ void store_nt(V v, void* p) { __builtin_nontemporal_store(v, static_cast<V*>(p)); }
-// Opaque to the compiler: a row kept in registers stays as it was loaded, not converted to fp32 (twice the registers)
-template <typename V>
-__device__ __forceinline__ void keep_as_is(V& v) {
-  typedef int i4 __attribute__((ext_vector_type(4)));
-  i4 w = __builtin_bit_cast(i4, v);
-  asm volatile("" : "+v"(w));
-  v = __builtin_bit_cast(V, w);
-}
 
-template <typename T> struct Row8;  // 8 logits as they lie in memory
-template <> struct Row8<bf16> {
-  bf16x8 v;
-  __device__ __forceinline__ void load(const bf16* p) { v = load_nt<bf16x8_u>(p); }
-  __device__ __forceinline__ float get(int j) const { return bf2f(v[j]); }
-  __device__ __forceinline__ void set(int j, float x) { v[j] = f2bf(x); }
-  __device__ __forceinline__ void store(bf16* p) const { store_nt<bf16x8_u>(v, p); }
-  __device__ __forceinline__ void keep() { keep_as_is(v); }
-};
-template <> struct Row8<_Float16> {
-  half8 v;
-  __device__ __forceinline__ void load(const _Float16* p) { v = load_nt<half8_u>(p); }
+// 16 bytes of logits as they lie in memory: neighbouring lanes take neighbouring chunks (two 16-byte halves of 8 fp32
+// values a lane leave half-used cache lines between them: the gradient pass ran at 5.1 TB/s)
+template <typename T> struct Packed;
+template <> struct Packed<bf16> { typedef bf16x8_u V; };
+template <> struct Packed<_Float16> { typedef half8_u V; };
+template <> struct Packed<float> { typedef f32x4_u V; };
+template <typename T>
+struct Chunk {
+  static constexpr int W = 16 / sizeof(T);
+  typedef typename Packed<T>::V V;
+  V v;
   __device__ __forceinline__ float get(int j) const { return (float)v[j]; }
-  __device__ __forceinline__ void set(int j, float x) { v[j] = (_Float16)x; }
-  __device__ __forceinline__ void store(_Float16* p) const { store_nt<half8_u>(v, p); }
-  __device__ __forceinline__ void keep() { keep_as_is(v); }
-};
-template <> struct Row8<float> {
-  f32x4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = load_nt<f32x4_u>(p);
-    b = load_nt<f32x4_u>(p + 4);
-  }
-  __device__ __forceinline__ float get(int j) const { return j < 4 ? a[j & 3] : b[j & 3]; }
-  __device__ __forceinline__ void set(int j, float x) {
-    if (j < 4) a[j & 3] = x;
-    else b[j & 3] = x;
-  }
-  __device__ __forceinline__ void store(float* p) const {
-    store_nt<f32x4_u>(a, p);
-    store_nt<f32x4_u>(b, p + 4);
-  }
+  __device__ __forceinline__ void set(int j, float x) { v[j] = (T)x; }
+  // opaque to the compiler: a row kept in registers stays as it was loaded, not converted to fp32 (twice the registers)
   __device__ __forceinline__ void keep() {
-    keep_as_is(a);
-    keep_as_is(b);
+    typedef int i4 __attribute__((ext_vector_type(4)));
+    i4 w = __builtin_bit_cast(i4, v);
+    asm volatile("" : "+v"(w));
+    v = __builtin_bit_cast(V, w);
+  }
+  // at logit c of a row (rows are below 2^28: byte offsets are 32-bit, one register beside the row's scalar base)
+  __device__ __forceinline__ void load(const T* x, int c) {
+    v = load_nt<V>(reinterpret_cast<const char*>(x) + (unsigned)c * (unsigned)sizeof(T));
+  }
+  __device__ __forceinline__ void store(T* x, int c) const {
+    store_nt<V>(v, reinterpret_cast<char*>(x) + (unsigned)c * (unsigned)sizeof(T));
   }
 };
-// the chunk [c, c + 8) of a row of V: past the end -inf on loads, left alone on stores
+// A row of V is V / W whole chunks and up to W - 1 logits behind them, which the workgroup's first lanes take one each
+// (handled in every chunk instead, the one-pass kernel grew past the instruction cache).
 template <typename T>
-__device__ __forceinline__ void load_chunk(Row8<T>& r, const T* x, int c, int V) {
-  if (c <= V - 8) {  // (V is below 2^31 - 2^16: offsets within a row are 32-bit)
-    r.load(x + c);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) r.set(j, c + j < V ? (float)x[c + j] : -INFINITY);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store_chunk(const Row8<T>& r, T* x, int c, int V) {
-  if (c <= V - 8) {
-    r.store(x + c);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < V) x[c + j] = (T)r.get(j);
-  }
-}
+__device__ __forceinline__ int whole(int V) { return V & ~(Chunk<T>::W - 1); }
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -109,14 +76,25 @@ struct Scale {  // c = log2(e) / temperature in two floats, both positive (d = -
   __device__ __forceinline__ float of_exp(float d) const { return exp2_(of(d)); }
 };
 
-// The sum of 2^((z - m) c) over 8 logits, pair by pair: the largest term (often near the whole sum) meets 3 roundings
-// here, not one for each term that follows it
+// The sum of 2^((z - m) c) over a chunk, pair by pair: the largest term (often near the whole sum) meets 2 or 3
+// roundings here, not one for each term that follows it
 template <typename T>
-__device__ __forceinline__ float exp_sum8(const Row8<T>& r, float m, const Scale& c) {
-  float e[8];
+__device__ __forceinline__ float exp_sum(const Chunk<T>& r, float m, const Scale& c) {
+  float e[Chunk<T>::W];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) e[j] = c.of_exp(r.get(j) - m);
-  return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+  for (int j = 0; j < Chunk<T>::W; ++j) e[j] = c.of_exp(r.get(j) - m);
+#pragma unroll
+  for (int n = Chunk<T>::W / 2; n > 0; n >>= 1)
+#pragma unroll
+    for (int j = 0; j < n; ++j) e[j] += e[j + n];
+  return e[0];
+}
+
+// (m, s) with one more logit (-inf: none)
+__device__ __forceinline__ void add_one(float x, const Scale& c, float* m, float* s) {
+  const float mn = fmaxf(*m, x), ms = mn == -INFINITY ? 0.f : mn;
+  *s = *s * c.of_exp(*m - ms) + c.of_exp(x - ms);
+  *m = mn;
 }
 
 // [B, S, V] logits (rows of unit inner stride) and the [B, S] per-token arrays that go with them
@@ -198,44 +176,43 @@ __device__ __forceinline__ RowSum block_join(float m, float s, const Scale& c) {
 template <typename T>
 __global__ void __launch_bounds__(kLseThreads) lse_partial_kernel(Logits L, Scale c, int pieces, int span,
                                                                   RowSum* __restrict__ part) {
-  constexpr int NW = kLseThreads / 64, U = sizeof(T) == 4 ? 2 : 4;
+  constexpr int NW = kLseThreads / 64, U = 4, W = Chunk<T>::W, STEP = kLseThreads * W;
   const int64_t row = blockIdx.x / pieces;
   const int64_t b = row / L.S, s0 = row % L.S;
   if (L.target_of(b, s0) < 0) return;
   const T* x = L.row<T>(b, s0);
-  const int begin = (int)(blockIdx.x % pieces) * span, end = (int)min((int64_t)begin + span, L.V);
+  const int V = (int)L.V, begin = (int)(blockIdx.x % pieces) * span, end = min(begin + span, whole<T>(V));
   float m = -INFINITY, s = 0.f;
-  for (int c0 = begin + threadIdx.x * 8; c0 < end; c0 += kLseThreads * 8 * U) {
-    Row8<T> r[U];
+  for (int c0 = begin + threadIdx.x * W; c0 < end; c0 += STEP * U) {
+    Chunk<T> r[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int cc = c0 + u * kLseThreads * 8;
-      if (cc < end) load_chunk(r[u], x, cc, end);
-    }
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * STEP < end) r[u].load(x, c0 + u * STEP);
     float mn = m;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (c0 + u * kLseThreads * 8 < end)
+      if (c0 + u * STEP < end)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) mn = fmaxf(mn, r[u].get(j));
+        for (int j = 0; j < W; ++j) mn = fmaxf(mn, r[u].get(j));
     const float ms = mn == -INFINITY ? 0.f : mn;  // nothing but -inf so far: the sum stays 0, not NaN
     float e = 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (c0 + u * kLseThreads * 8 < end) e += exp_sum8(r[u], ms, c);
+      if (c0 + u * STEP < end) e += exp_sum(r[u], ms, c);
     s = s * c.of_exp(m - ms) + e;
     m = mn;
   }
+  if (begin + span >= V && threadIdx.x < V - whole<T>(V)) add_one((float)x[whole<T>(V) + threadIdx.x], c, &m, &s);
   const RowSum all = block_join<NW>(m, s, c);
   if (threadIdx.x == 0) part[blockIdx.x] = all;
 }
 
-// Log-probability of token t from its row's (M, S), in fp64; a row of nothing but -inf, or with a NaN or +inf, gives NaN.
-template <typename T>
-__device__ __forceinline__ double row_logprob(const T* x, int64_t t, float M, double S, double inv_temp, float* l2s) {
+// Log-probability of the token with logit zt from its row's (M, S), in fp64; a row of nothing but -inf, or with a NaN or
+// +inf, gives NaN.
+__device__ __forceinline__ double row_logprob(float zt, float M, double S, double inv_temp, float* l2s) {
   const double l2 = log2(S);
   *l2s = (float)l2;
-  return ((double)(float)x[t] - (double)M) * inv_temp - l2 * 0.69314718055994530942;
+  return ((double)zt - (double)M) * inv_temp - l2 * 0.69314718055994530942;
 }
 
 // A group of `lanes` (a power of two, at least `pieces`) joins its row's pieces: (M, S) in every lane of the group
@@ -275,6 +252,27 @@ __device__ __forceinline__ void block_sums64(double (&v)[K]) {
   __syncthreads();
 }
 
+// f(b, sums of sequence b's segments) for every sequence, by one 256-thread workgroup: a thread a sequence where they have
+// few segments, a wave a sequence (f in its first lane) where they have many
+template <int K, typename F>
+__device__ __forceinline__ void for_each_sequence(const double* __restrict__ seg, int64_t B, int segs, F f) {
+  const bool waves = segs > 16;
+  const int lane = threadIdx.x & 63;
+  for (int64_t b = waves ? threadIdx.x >> 6 : threadIdx.x; b < B; b += waves ? 4 : 256) {
+    double q[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) q[k] = 0.0;
+    for (int i = waves ? lane : 0; i < segs; i += waves ? 64 : 1)
+#pragma unroll
+      for (int k = 0; k < K; ++k) q[k] += seg[(b * segs + i) * K + k];
+    if (waves) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) q[k] = wave_sum64(q[k]);
+    }
+    if (!waves || lane == 0) f(b, q);
+  }
+}
+
 // ------------------------------------------------------------------ token log-probabilities
 // 256 / lanes rows a workgroup, here and in the other passes over rows; the group's first lane does the row
 template <typename T>
@@ -289,7 +287,7 @@ __global__ void __launch_bounds__(256) logprob_rows_kernel(Logits L, const RowSu
   join_pieces(part, pieces, lanes, row, t >= 0, c, &st.M, &S);
   if (!there || (threadIdx.x & (lanes - 1))) return;
   if (t >= 0) {
-    lp = row_logprob(L.row<T>(b, s), t, st.M, S, inv_temp, &st.l2s);
+    lp = row_logprob((float)L.row<T>(b, s)[t], st.M, S, inv_temp, &st.l2s);
     st.coef = 1.f;
   }
   logp[row] = (float)lp;
@@ -302,19 +300,37 @@ struct PolicyArgs {
   double low, high, kl_coef;  // ratio bounds 1 - clip, 1 + clip_high
 };
 
+// A value that is the same in every lane, in a scalar register
+__device__ __forceinline__ float scalar(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+
+struct TokenInputs {
+  float old_logp, ref_logp, adv;
+  bool has_ref;
+  __device__ __forceinline__ void to_scalar() {
+    old_logp = scalar(old_logp);
+    ref_logp = scalar(ref_logp);
+    adv = scalar(adv);
+  }
+  __device__ __forceinline__ TokenInputs(const PolicyArgs& a, int64_t b, int64_t s)
+      : old_logp(a.old_logp.at(b, s)), ref_logp(a.ref_logp.p ? a.ref_logp.at(b, s) : 0.f), adv(a.adv.at(b, s)),
+        has_ref(a.ref_logp.p != nullptr) {}
+};
+
 // One token: the loss term, and its slope by lp.  min(r A, clip(r) A) has slope r A except where the clipped term is the
 // smaller one: A > 0 above the upper bound, A < 0 below the lower one.
-__device__ __forceinline__ void policy_token(const PolicyArgs& a, int64_t b, int64_t s, double lp, double* loss,
+__device__ __forceinline__ void policy_token(const PolicyArgs& a, const TokenInputs& in, double lp, double* loss,
                                              double* slope, double* kl, bool* clipped) {
-  const double A = (double)a.adv.at(b, s);
-  const double r = exp(lp - (double)a.old_logp.at(b, s));
+  const double A = (double)in.adv;
+  const double r = exp(lp - (double)in.old_logp);
   *clipped = (A > 0.0 && r > a.high) || (A < 0.0 && r < a.low);
   const double rc = *clipped ? (A > 0.0 ? a.high : a.low) : r;
   *loss = -rc * A;
   *slope = *clipped ? 0.0 : -r * A;
   *kl = 0.0;
-  if (a.ref_logp.p) {
-    const double d = (double)a.ref_logp.at(b, s) - lp;
+  if (in.has_ref) {
+    const double d = (double)in.ref_logp - lp;
     const double e = expm1(d);
     *kl = e - d;
     if (a.kl_coef != 0.0) {
@@ -339,10 +355,10 @@ __global__ void __launch_bounds__(256) policy_rows_kernel(Logits L, const RowSum
   join_pieces(part, pieces, lanes, row, t >= 0, c, &st.M, &S);
   if (s < L.S && (threadIdx.x & (lanes - 1)) == 0) {
     if (t >= 0) {
-      lp = row_logprob(L.row<T>(b, s), t, st.M, S, inv_temp, &st.l2s);
+      lp = row_logprob((float)L.row<T>(b, s)[t], st.M, S, inv_temp, &st.l2s);
       double slope;
       bool clipped;
-      policy_token(a, b, s, lp, &v[0], &slope, &v[1], &clipped);
+      policy_token(a, TokenInputs(a, b, s), lp, &v[0], &slope, &v[1], &clipped);
       v[2] = clipped ? 1.0 : 0.0;
       v[3] = 1.0;
       st.coef = (float)slope;
@@ -355,26 +371,18 @@ __global__ void __launch_bounds__(256) policy_rows_kernel(Logits L, const RowSum
 }
 
 // stats: {kl, clip fraction}; weight[b]: what a token of sequence b counts in the loss
-__global__ void __launch_bounds__(256) policy_total_kernel(const double4* __restrict__ seg, int64_t B, int segs,
+__global__ void __launch_bounds__(256) policy_total_kernel(const double* __restrict__ seg, int64_t B, int segs,
                                                            int by_sequence, double scale, float* __restrict__ loss,
                                                            float* __restrict__ stats, float* __restrict__ weight) {
   double v[4] = {0.0, 0.0, 0.0, 0.0};
-  for (int64_t b = threadIdx.x; b < B; b += 256) {
-    double q[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int i = 0; i < segs; ++i) {
-      const double4 x = seg[b * segs + i];
-      q[0] += x.x;
-      q[1] += x.y;
-      q[2] += x.z;
-      q[3] += x.w;
-    }
+  for_each_sequence<4>(seg, B, segs, [&](int64_t b, double (&q)[4]) {
     if (by_sequence) {
       const double w = 1.0 / ((q[3] > 1.0 ? q[3] : 1.0) * (double)B);
       q[0] *= w;
       weight[b] = (float)(w * scale);
     }
     for (int k = 0; k < 4; ++k) v[k] += q[k];
-  }
+  });
   block_sums64(v);
   const double w = 1.0 / (v[3] > 1.0 ? v[3] : 1.0);
   if (!by_sequence)
@@ -401,7 +409,7 @@ __global__ void __launch_bounds__(256) pair_rows_kernel(Logits L, const RowSum* 
   join_pieces(part, pieces, lanes, row, t >= 0, c, &st.M, &S);
   if (s < L.S && (threadIdx.x & (lanes - 1)) == 0) {
     if (t >= 0) {
-      v[0] = row_logprob(L.row<T>(b, s), t, st.M, S, 1.0, &st.l2s);
+      v[0] = row_logprob((float)L.row<T>(b, s)[t], st.M, S, 1.0, &st.l2s);
       v[1] = 1.0;
       st.coef = 1.f;
     }
@@ -411,34 +419,30 @@ __global__ void __launch_bounds__(256) pair_rows_kernel(Logits L, const RowSum* 
   if (threadIdx.x == 0) seg[blockIdx.x] = make_double2(v[0], v[1]);
 }
 
-// Pair p: sequences p (chosen) and p + P (rejected).  softplus(x) = max(x, 0) + log1p(exp(-|x|)).
-__global__ void __launch_bounds__(256) pair_total_kernel(const double2* __restrict__ seg, int64_t P, int segs,
+// Pair p: sequences p (chosen) and p + P (rejected).  softplus(x) = max(x, 0) + log1p(exp(-|x|)).  total: [2 P] scratch.
+__global__ void __launch_bounds__(256) pair_total_kernel(const double* __restrict__ seg, int64_t P, int segs,
                                                          const float* __restrict__ ref, int64_t ref_stride,
                                                          double beta, double smoothing, int average, double scale,
-                                                         float* __restrict__ loss, float* __restrict__ logp,
-                                                         float* __restrict__ margin, float* __restrict__ weight) {
+                                                         double2* __restrict__ total, float* __restrict__ loss,
+                                                         float* __restrict__ logp, float* __restrict__ margin,
+                                                         float* __restrict__ weight) {
+  for_each_sequence<2>(seg, 2 * P, segs, [&](int64_t b, double (&q)[2]) {
+    const double share = average ? 1.0 / (q[1] > 1.0 ? q[1] : 1.0) : 1.0;
+    logp[b] = (float)(q[0] * share);
+    total[b] = make_double2(q[0] * share, share);
+  });
+  __syncthreads();
   double v[1] = {0.0};
   for (int64_t p = threadIdx.x; p < P; p += 256) {
-    double gap[2], share[2];
-    for (int side = 0; side < 2; ++side) {
-      const int64_t b = p + side * P;
-      double l = 0.0, n = 0.0;
-      for (int i = 0; i < segs; ++i) {
-        l += seg[b * segs + i].x;
-        n += seg[b * segs + i].y;
-      }
-      share[side] = average ? 1.0 / (n > 1.0 ? n : 1.0) : 1.0;
-      l *= share[side];
-      logp[b] = (float)l;
-      gap[side] = ref ? l - (double)ref[b * ref_stride] : l;
-    }
-    const double h = beta * (gap[0] - gap[1]);
+    const double2 yes = total[p], no = total[p + P];
+    const double r = ref ? (double)ref[p * ref_stride] - (double)ref[(p + P) * ref_stride] : 0.0;
+    const double h = beta * (yes.x - no.x - r);
     const double tail = log1p(exp(-fabs(h)));
     v[0] += (1.0 - smoothing) * (tail + (h < 0.0 ? -h : 0.0)) + smoothing * (tail + (h > 0.0 ? h : 0.0));
     margin[p] = (float)h;
     const double slope = scale * beta / (double)P * (1.0 / (1.0 + exp(-h)) - (1.0 - smoothing));
-    weight[p] = (float)(slope * share[0]);
-    weight[p + P] = (float)(-slope * share[1]);
+    weight[p] = (float)(slope * yes.y);
+    weight[p + P] = (float)(-slope * no.y);
   }
   block_sums64(v);
   if (threadIdx.x == 0) *loss = (float)(scale * v[0] / (double)P);
@@ -446,34 +450,48 @@ __global__ void __launch_bounds__(256) pair_total_kernel(const double2* __restri
 
 // ------------------------------------------------------------------ gradient of the logits
 constexpr int kGradThreads = 256, kGradChunks = 4;
-constexpr int kGradSpan = kGradThreads * kGradChunks * 8;  // logits of one workgroup
+template <typename T> constexpr int kGradSpan = kGradThreads * kGradChunks * Chunk<T>::W;  // logits of one workgroup
 
-// dz of the chunks [begin, begin + CHUNKS * NT * 8) of a row that are in registers
+// -k 2^((z - M) c - log2 s): dz without the k that the target's logit gets on top
+__device__ __forceinline__ float grad_of(float z, float M, float l2s, float k, const Scale& c) {
+  const float d = z - M;
+  return exp2_(fmaf(d, c.hi, fmaf(d, c.lo, -l2s))) * -k;
+}
+// dz of the whole chunks [begin, begin + CHUNKS * NT * W) of a row that are in registers
 template <typename T, int CHUNKS, int NT>
-__device__ __forceinline__ void write_grad(Row8<T> (&r)[CHUNKS], T* out, int begin, int V, int t, float M,
-                                           float l2s, float k, const Scale& c) {
+__device__ __forceinline__ void write_grad(Chunk<T> (&r)[CHUNKS], T* out, int begin, int V, float M, float l2s, float k,
+                                           const Scale& c) {
+  constexpr int W = Chunk<T>::W;
 #pragma unroll
   for (int u = 0; u < CHUNKS; ++u) {
-    const int cc = begin + (u * NT + (int)threadIdx.x) * 8;
-    if (cc < V) {
+    const int cc = begin + (u * NT + (int)threadIdx.x) * W;
+    if (cc < whole<T>(V)) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float d = r[u].get(j) - M, p = exp2_(fmaf(d, c.hi, fmaf(d, c.lo, -l2s)));
-        r[u].set(j, ((cc + j == t ? 1.f : 0.f) - p) * k);
-      }
-      store_chunk(r[u], out, cc, V);
+      for (int j = 0; j < W; ++j) r[u].set(j, grad_of(r[u].get(j), M, l2s, k, c));
+      r[u].store(out, cc);
     }
+    __builtin_amdgcn_sched_barrier(0);  // one chunk's fp32 values at a time: registers
+  }
+}
+// The target's logit once more, with its k: one value a row, where a comparison in every element would be a sixth of the
+// pass's arithmetic.  By the lane that wrote its chunk, so that the two stores are in order.
+template <typename T, int NT>
+__device__ __forceinline__ void write_target(T* out, int V, int t, float zt, float M, float l2s, float k, const Scale& c) {
+  const int owner = t < whole<T>(V) ? t / Chunk<T>::W % NT : t - whole<T>(V);
+  if ((int)threadIdx.x == owner) {
+    const float d = zt - M;
+    out[t] = (T)((1.f - exp2_(fmaf(d, c.hi, fmaf(d, c.lo, -l2s)))) * k);
   }
 }
 template <typename T, int CHUNKS, int NT>
 __device__ __forceinline__ void write_zeros(T* out, int begin, int V) {
-  Row8<T> zero;
+  Chunk<T> zero;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) zero.set(j, 0.f);
+  for (int j = 0; j < Chunk<T>::W; ++j) zero.set(j, 0.f);
 #pragma unroll
   for (int u = 0; u < CHUNKS; ++u) {
-    const int cc = begin + (u * NT + (int)threadIdx.x) * 8;
-    if (cc < V) store_chunk(zero, out, cc, V);
+    const int cc = begin + (u * NT + (int)threadIdx.x) * Chunk<T>::W;
+    if (cc < whole<T>(V)) zero.store(out, cc);
   }
 }
 
@@ -487,22 +505,29 @@ __global__ void __launch_bounds__(kGradThreads) logit_grad_kernel(Logits L, Scal
   if (unless_one && *gout.p == 1.f) return;
   for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
     const int64_t row = unit / spans, b = row / L.S, s0 = row % L.S;
-    const int begin = (int)(unit % spans) * kGradSpan, V = (int)L.V, t = (int)L.target_of(b, s0);
+    const int begin = (int)(unit % spans) * kGradSpan<T>, V = (int)L.V, t = (int)L.target_of(b, s0);
+    // the lane's logit behind the last whole chunk, where it has one and the span reaches there
+    const int last = whole<T>(V) + (int)threadIdx.x;
+    const bool tail = last < V && whole<T>(V) - begin < kGradSpan<T> && whole<T>(V) >= begin;
     T* out = dz + row * L.V;
     if (t < 0) {
       write_zeros<T, kGradChunks, kGradThreads>(out, begin, V);
+      if (tail) out[last] = (T)0.f;
       continue;
     }
     const T* x = L.row<T>(b, s0);
-    Row8<T> r[kGradChunks];
+    Chunk<T> r[kGradChunks];
 #pragma unroll
     for (int u = 0; u < kGradChunks; ++u) {
-      const int cc = begin + (u * kGradThreads + (int)threadIdx.x) * 8;
-      if (cc < V) load_chunk(r[u], x, cc, V);
+      const int cc = begin + (u * kGradThreads + (int)threadIdx.x) * Chunk<T>::W;
+      if (cc < whole<T>(V)) r[u].load(x, cc);
     }
     const RowState st = rows[row];
     const float k = st.coef * (weight ? weight[b] : 1.f) * gout.at(b, s0) * inv_temp;
-    write_grad<T, kGradChunks, kGradThreads>(r, out, begin, V, t, st.M, st.l2s, k, c);
+    write_grad<T, kGradChunks, kGradThreads>(r, out, begin, V, st.M, st.l2s, k, c);
+    if (tail) out[last] = (T)grad_of((float)x[last], st.M, st.l2s, k, c);
+    if (t >= begin && t - begin < kGradSpan<T>)
+      write_target<T, kGradThreads>(out, V, t, (float)x[t], st.M, st.l2s, k, c);
   }
 }
 
@@ -511,39 +536,76 @@ __global__ void __launch_bounds__(kGradThreads) logit_grad_kernel(Logits L, Scal
 // weight[b] = scale / tokens, or scale / (B * tokens of b); count[0] = tokens
 __global__ void __launch_bounds__(1024) policy_weight_kernel(Logits L, int by_sequence, double scale,
                                                              float* __restrict__ weight, double* __restrict__ count) {
-  __shared__ double red[16];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  int64_t all = 0;  // of this wave
-  for (int64_t b = wave; b < L.B; b += 16) {
-    int64_t n = 0;
-    for (int64_t s = lane; s < L.S; s += 64) n += L.target_of(b, s) >= 0 ? 1 : 0;
+  const int lane = threadIdx.x & 63;
+  double v[1] = {0.0};  // of this thread
+  if (by_sequence && L.B >= 16) {  // a wave a sequence
+    for (int64_t b = threadIdx.x >> 6; b < L.B; b += 16) {
+      int n = 0;
+      for (int64_t s = lane; s < L.S; s += 64) n += L.target_of(b, s) >= 0 ? 1 : 0;
+      v[0] += (double)n;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, kWave);
-    if (by_sequence && lane == 0) weight[b] = (float)(scale / ((double)(n > 1 ? n : 1) * (double)L.B));
-    all += n;
+      for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, kWave);
+      if (lane == 0) weight[b] = (float)(scale / ((double)(n > 1 ? n : 1) * (double)L.B));
+    }
+  } else if (by_sequence) {  // all of them a sequence
+    for (int64_t b = 0; b < L.B; ++b) {
+      double n[1] = {0.0};
+      for (int64_t s = threadIdx.x; s < L.S; s += 1024) n[0] += L.target_of(b, s) >= 0 ? 1.0 : 0.0;
+      v[0] += n[0];
+      block_sums64<1, 16>(n);
+      if (threadIdx.x == 0) weight[b] = (float)(scale / ((n[0] > 1.0 ? n[0] : 1.0) * (double)L.B));
+    }
+  } else {
+    int n = 0;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < L.B * L.S; i += 1024) n += L.target_of(i / L.S, i % L.S) >= 0 ? 1 : 0;
+    v[0] = (double)n;
   }
-  if (lane == 0) red[wave] = (double)all;
-  __syncthreads();
-  double n = 0.0;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) n += red[w];
+  block_sums64<1, 16>(v);
   if (!by_sequence)
-    for (int64_t b = threadIdx.x; b < L.B; b += 1024) weight[b] = (float)(scale / (n > 1.0 ? n : 1.0));
-  if (threadIdx.x == 0) *count = n;
+    for (int64_t b = threadIdx.x; b < L.B; b += 1024) weight[b] = (float)(scale / (v[0] > 1.0 ? v[0] : 1.0));
+  if (threadIdx.x == 0) *count = v[0];
 }
 
-// One workgroup a row, the row in registers between its two uses (CHUNKS * NT * 8 logits at least V): one read and
-// one write of the logits' size.  terms[row]: {weighted loss, kl, clipped}.
-template <typename T, int NT, int CHUNKS, int WAVES>  // WAVES a SIMD that the registers have to leave room for
+// Running (m, s) of a thread over its chunks of a row
+template <typename T, int NT, int N>
+__device__ __forceinline__ void add_chunks(Chunk<T> (&r)[N], int V, const Scale& c, float* m, float* s) {
+  constexpr int W = Chunk<T>::W, G = 16 / W;  // G chunks share a rescaling
+#pragma unroll
+  for (int g = 0; g < N; g += G) {
+    float mn = *m;
+#pragma unroll
+    for (int u = g; u < (g + G < N ? g + G : N); ++u)
+      if ((u * NT + (int)threadIdx.x) * W < whole<T>(V))
+#pragma unroll
+        for (int j = 0; j < W; ++j) mn = fmaxf(mn, r[u].get(j));
+    const float ms = mn == -INFINITY ? 0.f : mn;
+    float e = 0.f;
+#pragma unroll
+    for (int u = g; u < (g + G < N ? g + G : N); ++u)
+      if ((u * NT + (int)threadIdx.x) * W < whole<T>(V)) e += exp_sum(r[u], ms, c);
+    *s = *s * c.of_exp(*m - ms) + e;
+    *m = mn;
+    __builtin_amdgcn_sched_barrier(0);  // one group's fp32 values at a time: registers
+  }
+#pragma unroll
+  for (int u = 0; u < N; ++u) r[u].keep();
+}
+// One workgroup a row, the row in registers between its two uses (NT * CHUNKS chunks, at least the row's): one read and
+// one write of the logits' size.  terms[row]: {weighted loss, kl, clipped}.  It ran at 4.6-5.1 TB/s until less arithmetic
+// and fewer registers a row brought 5.6-5.9 of the copy's 6.1; what is left is the time that a row's terms keep its
+// workgroup waiting.
+template <typename T, int NT, int CHUNKS, int WAVES>  // WAVES a SIMD that the registers leave room for
 __global__ void __launch_bounds__(NT, WAVES) policy_fused_kernel(Logits L, Scale c, double inv_temp, PolicyArgs a,
-                                                          const float* __restrict__ weight, float* __restrict__ logp,
-                                                          RowState* __restrict__ rows, double4* __restrict__ terms,
-                                                          T* __restrict__ dz) {
+                                                                 const float* __restrict__ weight,
+                                                                 float* __restrict__ logp, RowState* __restrict__ rows,
+                                                                 double4* __restrict__ terms, T* __restrict__ dz) {
   const int64_t row = blockIdx.x, b = row / L.S, s0 = row % L.S;
-  const int V = (int)L.V, t = (int)L.target_of(b, s0);
+  const int V = (int)L.V, t = (int)L.target_of(b, s0), last = whole<T>(V) + (int)threadIdx.x;
   T* out = dz + row * L.V;
   if (t < 0) {
     write_zeros<T, CHUNKS, NT>(out, 0, V);
+    if (last < V) out[last] = (T)0.f;
     if (threadIdx.x == 0) {
       logp[row] = 0.f;
       rows[row] = RowState{0.f, 0.f, 0.f, 0.f};
@@ -552,42 +614,31 @@ __global__ void __launch_bounds__(NT, WAVES) policy_fused_kernel(Logits L, Scale
     return;
   }
   const T* x = L.row<T>(b, s0);
-  Row8<T> r[CHUNKS];
+  // what the row's terms need is requested first: thread 0 works on them while all the others wait
+  TokenInputs in(a, b, s0);
+  float zt = (float)x[t], w = weight[b];
+  const float tail = last < V ? (float)x[last] : -INFINITY;
+  Chunk<T> r[CHUNKS];
 #pragma unroll
   for (int u = 0; u < CHUNKS; ++u) {  // every load in flight before any use
-    const int cc = (u * NT + (int)threadIdx.x) * 8;
-    if (cc < V) load_chunk(r[u], x, cc, V);
+    const int cc = (u * NT + (int)threadIdx.x) * Chunk<T>::W;
+    if (cc < whole<T>(V)) r[u].load(x, cc);
   }
+  in.to_scalar();
+  zt = scalar(zt);
+  w = scalar(w);
   float m = -INFINITY, s = 0.f;
-  constexpr int G = 2;  // chunks that share a rescaling
-#pragma unroll
-  for (int g = 0; g < CHUNKS; g += G) {
-    float mn = m;
-#pragma unroll
-    for (int u = g; u < (g + G < CHUNKS ? g + G : CHUNKS); ++u)
-      if ((u * NT + (int)threadIdx.x) * 8 < V)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mn = fmaxf(mn, r[u].get(j));
-    const float ms = mn == -INFINITY ? 0.f : mn;
-    float e = 0.f;
-#pragma unroll
-    for (int u = g; u < (g + G < CHUNKS ? g + G : CHUNKS); ++u)
-      if ((u * NT + (int)threadIdx.x) * 8 < V) e += exp_sum8(r[u], ms, c);
-    s = s * c.of_exp(m - ms) + e;
-    m = mn;
-  }
-#pragma unroll
-  for (int u = 0; u < CHUNKS; ++u) r[u].keep();
+  add_chunks<T, NT>(r, V, c, &m, &s);
+  add_one(tail, c, &m, &s);
   __shared__ float pass[3];
   const RowSum all = block_join<NT / 64>(m, s, c);
   if (threadIdx.x == 0) {
     RowState st{all.M, 0.f, 0.f, 0.f};
-    const double lp = row_logprob(x, t, all.M, all.S, inv_temp, &st.l2s);
+    const double lp = row_logprob(zt, all.M, all.S, inv_temp, &st.l2s);
     double loss, slope, kl;
     bool clipped;
-    policy_token(a, b, s0, lp, &loss, &slope, &kl, &clipped);
+    policy_token(a, in, lp, &loss, &slope, &kl, &clipped);
     st.coef = (float)slope;
-    const float w = weight[b];
     pass[0] = st.M;
     pass[1] = st.l2s;
     pass[2] = st.coef * w * (float)inv_temp;
@@ -596,7 +647,10 @@ __global__ void __launch_bounds__(NT, WAVES) policy_fused_kernel(Logits L, Scale
     terms[row] = make_double4(loss * (double)w, kl, clipped ? 1.0 : 0.0, 0.0);
   }
   __syncthreads();
-  write_grad<T, CHUNKS, NT>(r, out, 0, V, t, pass[0], pass[1], pass[2], c);
+  const float M = pass[0], l2s = pass[1], k = pass[2];
+  write_grad<T, CHUNKS, NT>(r, out, 0, V, M, l2s, k, c);
+  if (last < V) out[last] = (T)grad_of(tail, M, l2s, k, c);
+  write_target<T, NT>(out, V, t, zt, M, l2s, k, c);
 }
 
 __global__ void __launch_bounds__(1024) policy_sum_kernel(const double4* __restrict__ terms, int64_t N,
@@ -626,7 +680,7 @@ struct LseShape {
 // Pieces of a row: enough workgroups to fill the chip where rows are few, each piece at least one round of loads;
 // lanes that join them: the next power of two
 static LseShape lse_shape(int64_t N, int64_t V) {
-  const int64_t least = kLseThreads * 8;
+  const int64_t least = kLseThreads * 8;  // one round of 16-bit loads, two of fp32
   int64_t pieces = N > 0 ? 2048 / N : 1;
   pieces = min(min(pieces, (V + least - 1) / least), (int64_t)kWave);
   if (pieces < 1) pieces = 1;
@@ -663,18 +717,18 @@ static Logits logits_of(const PrefLogits& l) {
 }
 static TokenArray array_of(const PrefTokens& t) { return {t.p, t.sb, t.ss}; }
 
-#define DTA_BY_TYPE(type, call)                     \
-  switch (type) {                                   \
-    case 0: { typedef float T; call; } break;       \
-    case 1: { typedef bf16 T; call; } break;        \
-    case 2: { typedef _Float16 T; call; } break;    \
-    default: return hipErrorInvalidValue;           \
+#define DTA_BY_TYPE(type, ...)                        \
+  switch (type) {                                     \
+    case 0: { typedef float T; __VA_ARGS__; } break;  \
+    case 1: { typedef bf16 T; __VA_ARGS__; } break;   \
+    case 2: { typedef _Float16 T; __VA_ARGS__; } break; \
+    default: return hipErrorInvalidValue;             \
   }
 
 // Workgroups of the passes over the logits have to fit a launch
 int dta_pref_fits(int64_t N, int64_t V) {
-  const int64_t most = (int64_t)1 << 31, spans = (V + kGradSpan - 1) / kGradSpan;
-  return N >= 0 && V > 0 && N < most && V < most - 65536 && N * spans < most;
+  const int64_t most = (int64_t)1 << 31, spans = (V + kGradSpan<float> - 1) / kGradSpan<float>;
+  return N >= 0 && V > 0 && N < most && V < ((int64_t)1 << 28) && N * spans < most;
 }
 int64_t dta_pref_parts(int64_t N, int64_t V) { return N * lse_shape(N, V).pieces; }
 int64_t dta_pref_segs(int64_t B, int64_t S, int64_t V) { return B * segments(S, lse_shape(B * S, V)); }
@@ -715,7 +769,7 @@ hipError_t dta_pref_policy(const PrefLogits& l, int type, double temperature, co
     })
     DTA_HIP_CHECK(hipGetLastError());
   }
-  hipLaunchKernelGGL(policy_total_kernel, dim3(1), dim3(256), 0, st, (double4*)seg, L.B, segs, p.by_sequence, p.scale,
+  hipLaunchKernelGGL(policy_total_kernel, dim3(1), dim3(256), 0, st, seg, L.B, segs, p.by_sequence, p.scale,
                      loss, stats, weight);
   return hipGetLastError();
 }
@@ -742,29 +796,29 @@ hipError_t dta_pref_policy_grad(const PrefLogits& l, int type, double temperatur
   double* count = terms + 4 * N;
   hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, L, p.by_sequence, p.scale, weight, count);
   DTA_HIP_CHECK(hipGetLastError());
+  // Threads and 16-byte chunks a thread by the row's size: as many rows on a CU as its registers hold (V = 50304 in bf16:
+  // 1024 x 7 at 8 waves a SIMD 279 us, 512 x 13 287, 256 x 25 306, 1024 x 7 at 4 waves 367, for 8192 rows)
 #define DTA_FUSED(T, NT, CHUNKS, WAVES) \
   policy_fused<T, NT, CHUNKS, WAVES>(L, temperature, p, weight, logp, rows, terms, dz, st)
-#define DTA_FUSED16(T)                                       \
-  if (L.V <= 256 * 8 * 4) DTA_FUSED(T, 256, 4, 8);           \
-  else if (L.V <= 256 * 8 * 8) DTA_FUSED(T, 256, 8, 5);      \
-  else if (L.V <= 512 * 8 * 8) DTA_FUSED(T, 512, 8, 5);      \
-  else if (L.V <= 512 * 8 * 13) DTA_FUSED(T, 512, 13, 4);    \
-  else if (L.V <= 1024 * 8 * 10) DTA_FUSED(T, 1024, 10, 4);  \
+#define DTA_FUSED_ANY(T, W)                                   \
+  if (L.V <= W * 64 * 2) DTA_FUSED(T, 64, 2, 8);              \
+  else if (L.V <= W * 256 * 2) DTA_FUSED(T, 256, 2, 8);       \
+  else if (L.V <= W * 256 * 4) DTA_FUSED(T, 256, 4, 8);       \
+  else if (L.V <= W * 512 * 4) DTA_FUSED(T, 512, 4, 8);       \
+  else if (L.V <= W * 1024 * 4) DTA_FUSED(T, 1024, 4, 8);     \
+  else if (L.V <= W * 1024 * 7) DTA_FUSED(T, 1024, 7, 8);     \
+  else if (L.V <= W * 512 * 16) DTA_FUSED(T, 512, 16, 4);     \
+  else if (L.V <= W * 1024 * 10) DTA_FUSED(T, 1024, 10, 4);   \
+  else if (L.V <= W * 1024 * 13) DTA_FUSED(T, 1024, 13, 4);   \
   else DTA_FUSED(T, 1024, 16, 4);
   if (type == 1) {
-    DTA_FUSED16(bf16)
+    DTA_FUSED_ANY(bf16, 8)
   } else if (type == 2) {
-    DTA_FUSED16(_Float16)
-  } else if (L.V <= 256 * 8 * 4) {
-    DTA_FUSED(float, 256, 4, 5);
-  } else if (L.V <= 256 * 8 * 12) {
-    DTA_FUSED(float, 256, 12, 3);
-  } else if (L.V <= 512 * 8 * 13) {
-    DTA_FUSED(float, 512, 13, 3);
+    DTA_FUSED_ANY(_Float16, 8)
   } else {
-    DTA_FUSED(float, 1024, 8, 4);
+    DTA_FUSED_ANY(float, 4)
   }
-#undef DTA_FUSED16
+#undef DTA_FUSED_ANY
 #undef DTA_FUSED
   DTA_HIP_CHECK(hipGetLastError());
   hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(1024), 0, st, (double4*)terms, N, count, loss, stats);
@@ -787,8 +841,8 @@ hipError_t dta_pref_pairs(const PrefLogits& l, int type, const float* ref, int64
     })
     DTA_HIP_CHECK(hipGetLastError());
   }
-  hipLaunchKernelGGL(pair_total_kernel, dim3(1), dim3(256), 0, st, (double2*)seg, L.B / 2, segs, ref, ref_stride, beta,
-                     smoothing, average, scale, loss, logp, margin, weight);
+  hipLaunchKernelGGL(pair_total_kernel, dim3(1), dim3(256), 0, st, seg, L.B / 2, segs, ref, ref_stride, beta, smoothing,
+                     average, scale, (double2*)seg + L.B * segs, loss, logp, margin, weight);
   return hipGetLastError();
 }
 
@@ -797,11 +851,11 @@ hipError_t dta_pref_grad(const PrefLogits& l, int type, double temperature, cons
   const Logits L = logits_of(l);
   const int64_t N = L.B * L.S;
   if (N == 0) return hipSuccess;
-  const int spans = (int)((L.V + kGradSpan - 1) / kGradSpan);
-  const int64_t units = N * spans;
-  // (a launch that is expected to end at once is a small one, whose workgroups walk over the rows if they have to)
-  const int64_t grid = unless_one ? min(units, (int64_t)2048) : units;
   DTA_BY_TYPE(type, {
+    const int spans = (int)((L.V + kGradSpan<T> - 1) / kGradSpan<T>);
+    const int64_t units = N * spans;
+    // (a launch that is expected to end at once is a small one, whose workgroups walk over the rows if they have to)
+    const int64_t grid = unless_one ? min(units, (int64_t)2048) : units;
     hipLaunchKernelGGL(logit_grad_kernel<T>, dim3((unsigned)grid), dim3(kGradThreads), 0, st, L, scale_of(temperature),
                        (const RowState*)rows, weight, array_of(gout), (float)(1.0 / temperature), spans, units,
                        unless_one, (T*)dz);

@@ -68,7 +68,8 @@ def test_token_logprobs(B, S, V, dtype, temperature):
 @pytest.mark.parametrize("B,S,V", [(1, 1, 1), (2, 5, 9), (4, 3, 63), (3, 7, 257), (2, 4, 1003), (4, 2, 8193), (2, 5, 50257),
                                    (4, 2, 128256), (3, 300, 33), (2, 700, 4099), (1, 512, 1), (3, 257, 8192), (2, 300, 16383),
                                    (1, 520, 24577), (1, 515, 32767), (2, 257, 50257), (1, 512, 53248), (1, 514, 65535),
-                                   (1, 513, 70001), (4, 130, 128256)])
+                                   (1, 513, 70001), (4, 130, 128256), (1, 5000, 33), (20, 40, 65), (17, 30, 1100),
+                                   (600, 1, 4200), (3, 200, 60001)])
 @pytest.mark.parametrize("kl,high,reduction,scale", [(0.0, None, "token", 1.0), (0.1, 0.28, "sequence", 0.25)])
 def test_policy_loss(B, S, V, dtype, kl, high, reduction, scale):
     z, target, old, ref, adv = _case(B, S, V, dtype, seed=B + S + V)
@@ -104,7 +105,7 @@ def test_policy_loss(B, S, V, dtype, kl, high, reduction, scale):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B,S,V", [(2, 1, 1), (2, 5, 9), (4, 3, 63), (6, 7, 257), (4, 2, 8193), (4, 5, 50257), (2, 3, 128256),
-                                   (4, 300, 33), (2, 700, 4099)])
+                                   (4, 300, 33), (2, 700, 4099), (2, 4500, 17), (300, 2, 40)])
 @pytest.mark.parametrize("smoothing,average,use_ref", [(0.0, False, True), (0.1, True, False)])
 def test_preference_loss(B, S, V, dtype, smoothing, average, use_ref):
     z, target, *_ = _case(B, S, V, dtype, seed=B + S + V)
@@ -248,6 +249,22 @@ def test_nothing_counts_and_nothing_there():
         out = preference.policy_loss(z, target, none, none)
         assert lp.shape == target.shape and out.loss.item() == 0
         assert torch.autograd.grad(out.loss + lp.sum(), z)[0].shape == z.shape
+
+
+@pytest.mark.parametrize("B,S,V", [(1, 5000, 33), (4, 130, 2003), (2, 300, 50257)])
+def test_policy_loss_without_gradient(B, S, V):
+    """The forward alone (several passes, no gradient) against the forward with one: each within its bound of the definition."""
+    z, target, old, ref, adv = _case(B, S, V, torch.bfloat16)
+    e = oracle.stat_error(z.double())
+    with torch.no_grad():
+        a = preference.policy_loss(z, target, old, adv, ref, kl_coef=0.1)
+    b = preference.policy_loss(z.clone().requires_grad_(), target, old, adv, ref, kl_coef=0.1)
+    live = target != -100
+    n = live.sum()
+    steep = ((torch.exp(a.logp - old) * adv.abs() + 0.1 * torch.expm1(ref - a.logp).abs()) * live).double().sum() / n
+    assert (a.logp - b.logp).abs().max() <= 2 * e + 2.0 ** -23 * a.logp.abs().max()
+    assert abs(float(a.loss) - float(b.loss.detach())) <= float(steep) * 2.1 * e + 2.0 ** -23 * abs(float(a.loss))
+    assert a.clip_fraction == b.clip_fraction and not a.loss.requires_grad and b.loss.requires_grad
 
 
 def test_offsets_past_32_bits():
