@@ -320,6 +320,21 @@ struct GradList {
     numel.push_back(t.numel());
     type.push_back(type_);
   }
+  // Memory that is listed twice is kept once (two parameters may share a gradient): scaled twice it would depend on
+  // which workgroup comes first
+  void drop_repeats() {
+    std::unordered_set<const void*> seen;
+    size_t n = 0;
+    for (size_t i = 0; i < p.size(); ++i) {
+      if (numel[i] > 0 && !seen.insert(p[i]).second) continue;
+      p[n] = p[i];
+      numel[n] = numel[i];
+      type[n++] = type[i];
+    }
+    p.resize(n);
+    numel.resize(n);
+    type.resize(n);
+  }
 };
 
 GradList grads_arg(const std::vector<Tensor>& ts) {
@@ -355,11 +370,12 @@ std::tuple<Tensor, Tensor> grad_sumsq(const std::vector<Tensor>& grads) {
 }
 
 void grad_clip_(const std::vector<Tensor>& grads, const Tensor& sumsq, double max_norm) {
-  const GradList g = grads_arg(grads);
+  GradList g = grads_arg(grads);
+  g.drop_repeats();
   TORCH_CHECK(sumsq.device() == grads[0].device() && sumsq.scalar_type() == torch::kFloat64 && sumsq.numel() == 1,
               "sumsq: f64 scalar on the gradients' GPU");
   const at::DeviceGuard guard(grads[0].device());
-  ok(dta_grad_clip(g.p.data(), g.numel.data(), g.type.data(), (int)grads.size(), sumsq.data_ptr<double>(), max_norm,
+  ok(dta_grad_clip(g.p.data(), g.numel.data(), g.type.data(), (int)g.p.size(), sumsq.data_ptr<double>(), max_norm,
                    stream_on(grads[0])),
      "grad_clip");
   for (const auto& t : grads) t.unsafeGetTensorImpl()->bump_version();
@@ -370,10 +386,9 @@ void grad_clip_(const std::vector<Tensor>& grads, const Tensor& sumsq, double ma
 OptTensor clip_params_(const std::vector<Tensor>& params, double max_norm) {
   GradList g;
   std::vector<Tensor> grads;
-  std::unordered_set<const void*> seen;
   for (const auto& p : params) {
     const Tensor& t = p.grad();
-    if (!t.defined() || !seen.insert(p.unsafeGetTensorImpl()).second) continue;  // listed twice: clipped once
+    if (!t.defined()) continue;
     if (t.layout() != torch::kStrided || !t.is_cuda() || (!grads.empty() && t.device() != grads[0].device()) ||
         float_type(t) < 0 || !t.is_non_overlapping_and_dense())
       return c10::nullopt;
@@ -381,6 +396,7 @@ OptTensor clip_params_(const std::vector<Tensor>& params, double max_norm) {
     grads.push_back(t);
   }
   if (grads.empty()) return c10::nullopt;
+  g.drop_repeats();  // a parameter listed twice, or a gradient that two share, counts and is clipped once
   const at::DeviceGuard guard(grads[0].device());
   const hipStream_t st = stream_on(grads[0]);
   const auto sn = sumsq_of(g, grads[0].device(), st);

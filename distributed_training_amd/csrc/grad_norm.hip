@@ -20,11 +20,11 @@ namespace dta {
 
 constexpr int kJobs = 160;       // 160 x 20 B of arguments stay under 4 KiB
 constexpr int kUnit = 8192;      // elements: 4 (2 bytes) to 16 (8 bytes) 16-byte loads a thread
-constexpr int kNormGrid = 2048;  // 8 workgroups on each of 256 CUs
+constexpr int kNormGrid = 8192;  // workgroups at most (1.4 G bf16 elements: 1459 us, 1514 with 2048, 1462 with 16384)
 
 // The norm's pass reads with non-temporal loads (6.9 TB/s, 5.4 without), except for what the Infinity Cache can hold
 // until the clipping pass: the last kKeep bytes, which that pass, walking each workgroup's run backwards, meets first.
-// Together, in us (bf16): 124 M elements PLACE_SMALL, 1.4 G PLACE_LARGE.
+// Norm and clip together, bf16: 124 M elements 128 us, 150 with nothing kept; 1.4 G 1513, 1529 with nothing kept.
 constexpr int64_t kKeep = 192 << 20;
 
 struct NormJobs {

@@ -105,7 +105,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     """Scale the parameters' gradients in place so that their global 2-norm is at most ``max_norm``, and return the
     norm before (a 0-dim fp32 tensor).  As ``torch.nn.utils.clip_grad_norm_`` with its 2-norm: the coefficient is
     ``min(1, max_norm / (norm + 1e-6))``, a NaN norm makes every gradient NaN; parameters without a gradient are
-    skipped.  On the GPU the norm is one pass over every gradient and the scaling another, left out on the device where the
+    skipped, and one that is listed twice (or a gradient that two share) counts and is scaled once.  On the GPU the norm is one pass over every gradient and the scaling another, left out on the device where the
     norm is within the bound: no host sync unless ``error_if_nonfinite`` asks for one.
 
     Gradients held by a DDP / FSDP engine: call the engine's own ``clip_grad_norm_``, which also sums over shards."""
@@ -116,10 +116,11 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
         norm = native().clip_params_(params, float(max_norm))  # one call for gradients that lie dense on one GPU
         if norm is not None:
             return norm
-    seen: Dict[int, torch.Tensor] = {}
-    for p in params:  # (a parameter listed twice is clipped once)
+    seen: Dict[Any, torch.Tensor] = {}
+    for p in params:
         if p.grad is not None:
-            seen.setdefault(id(p), p.grad)
+            key = (p.grad.data_ptr(), p.grad.device) if p.grad.numel() and p.grad.layout == torch.strided else id(p)
+            seen.setdefault(key, p.grad)
     grads = list(seen.values())
     if not grads:
         return torch.zeros(())

@@ -75,6 +75,12 @@ def _positive(x: float, name: str) -> float:
     return float(x)
 
 
+def _temperature(x: float) -> float:
+    if not 1e-6 <= x <= 1e6:
+        raise ValueError(f"temperature must be between 1e-6 and 1e6 (got {x})")
+    return float(x)
+
+
 def _not_negative(x: float, name: str) -> float:
     if not (x >= 0.0 and math.isfinite(x)):
         raise ValueError(f"{name} must be finite and not negative (got {x})")
@@ -100,7 +106,7 @@ def token_logprobs(logits: torch.Tensor, target: torch.Tensor, ignore_index: int
                    temperature: float = 1.0) -> torch.Tensor:
     """``log softmax(logits / temperature)`` at each position's target: fp32, of ``target``'s shape, 0 where a position
     does not count.  What a rollout stores as ``old_logp`` and a frozen model gives as ``ref_logp``; differentiable."""
-    temperature = _positive(temperature, "temperature")
+    temperature = _temperature(temperature)
     if logits.is_cuda:
         return native().token_logprobs(logits, target, ignore_index, temperature)
     _check(logits, target)
@@ -156,7 +162,7 @@ def policy_loss(logits: torch.Tensor, target: torch.Tensor, old_logp: torch.Tens
     accumulation pass 1 / steps here rather than dividing the result.  No token counting: the loss is 0."""
     clip, kl_coef = _not_negative(clip, "clip"), _not_negative(kl_coef, "kl_coef")
     clip_high = clip if clip_high is None else _not_negative(clip_high, "clip_high")
-    temperature = _positive(temperature, "temperature")
+    temperature = _temperature(temperature)
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite (got {scale})")
     if reduction not in ("token", "sequence"):

@@ -89,6 +89,20 @@ def test_layouts():
     assert torch.equal(wide[:, :7], keep[:, :7]) and torch.equal(wide[:, 27:], keep[:, 27:])
 
 
+def test_what_is_listed_twice_is_clipped_once():
+    p, q = _params([4000, 4000], [torch.float32])
+    q.grad = p.grad
+    before = p.grad.double().clone()
+    norm = float(before.square().sum().sqrt())
+    for params in ([p, q], [p, p, q]):
+        p.grad.copy_(before)
+        assert abs(float(optim.clip_grad_norm_(params, 0.5)) - norm) <= 2.0 ** -23 * norm
+        assert ((p.grad.double() - before * (0.5 / (norm + 1e-6))).abs() <= before.abs() * 2.0 ** -22).all()
+    optim.grad_clip_([p.grad, p.grad], optim.grad_sumsq([p.grad])[0], 0.25)
+    want = before * (0.25 / norm)
+    assert ((p.grad.double() - want).abs() <= want.abs() * 1e-5).all()
+
+
 def test_extremes_and_nonfinite():
     assert abs(float(optim.global_norm(torch.full((10000,), 1e25, device=DEV))) / 1e27 - 1) < 1e-6
     assert abs(float(optim.global_norm(torch.full((10000,), 1e-30, device=DEV))) / 1e-28 - 1) < 1e-6

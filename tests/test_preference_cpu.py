@@ -122,8 +122,11 @@ def test_refusals():
     with pytest.raises(TypeError, match="floating"):
         T(z.long(), target)
     for bad in (0.0, -1.0, float("nan"), float("inf")):
-        with pytest.raises(ValueError, match="temperature"):
-            T(z, target, temperature=bad)
+        for t in (bad, 1e-7, 1e7):
+            with pytest.raises(ValueError, match="temperature"):
+                T(z, target, temperature=t)
+            with pytest.raises(ValueError, match="temperature"):
+                P(z, target, old, adv, temperature=t)
         with pytest.raises(ValueError, match="beta"):
             R(z, target, beta=bad)
     with pytest.raises(ValueError, match="old_logp must be"):

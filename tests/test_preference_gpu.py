@@ -238,9 +238,10 @@ def test_nothing_counts_and_nothing_there():
         out = preference.policy_loss(z, target, nan, nan, nan, kl_coef=0.1, reduction=reduction)
         assert out.loss.item() == 0 and out.kl.item() == 0 and out.clip_fraction.item() == 0
         assert (torch.autograd.grad(out.loss, z)[0] == 0).all()
-    out = preference.preference_loss(z, target)
-    assert abs(out.loss.item() - math.log(2)) < 1e-6 and (out.margin == 0).all()
-    assert (torch.autograd.grad(out.loss, z)[0] == 0).all()
+    for x, t in ((z, target), (torch.randn(2, 0, 50, device=DEV, requires_grad=True), target[:, :0])):
+        out = preference.preference_loss(x, t)
+        assert abs(out.loss.item() - math.log(2)) < 1e-6 and (out.margin == 0).all()
+        assert (torch.autograd.grad(out.loss, x)[0] == 0).all()
     for shape in ((2, 0, 50), (0, 50)):
         z = torch.randn(shape, device=DEV, requires_grad=True)
         target = torch.zeros(shape[:-1], dtype=torch.long, device=DEV)
