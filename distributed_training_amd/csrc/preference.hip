@@ -104,6 +104,9 @@ struct Logits {
   const int64_t* target;
   int64_t tb, ts;
   int64_t B, S, V, ignore;
+  // rows are counted in 32 bits (B * S is below 2^31): a 64-bit division is a hundred instructions
+  __device__ __forceinline__ int64_t sequence_of(unsigned row) const { return row / (unsigned)S; }
+  __device__ __forceinline__ int64_t token_of(unsigned row) const { return row % (unsigned)S; }
   template <typename T>
   __device__ __forceinline__ const T* row(int64_t b, int64_t s) const {
     return static_cast<const T*>(z) + b * sb + s * ss;
@@ -178,11 +181,11 @@ template <typename T>
 __global__ void __launch_bounds__(kLseThreads) lse_partial_kernel(Logits L, Scale c, int pieces, int span,
                                                                   RowSum* __restrict__ part) {
   constexpr int NW = kLseThreads / 64, U = 4, W = Chunk<T>::W, STEP = kLseThreads * W;
-  const int64_t row = blockIdx.x / pieces;
-  const int64_t b = row / L.S, s0 = row % L.S;
+  const unsigned row = blockIdx.x / (unsigned)pieces;
+  const int64_t b = L.sequence_of(row), s0 = L.token_of(row);
   if (L.target_of(b, s0) < 0) return;
   const T* x = L.row<T>(b, s0);
-  const int V = (int)L.V, begin = (int)(blockIdx.x % pieces) * span, end = min(begin + span, whole<T>(V));
+  const int V = (int)L.V, begin = (int)(blockIdx.x % (unsigned)pieces) * span, end = min(begin + span, whole<T>(V));
   float m = -INFINITY, s = 0.f;
   for (int c0 = begin + threadIdx.x * W; c0 < end; c0 += STEP * U) {
     Chunk<T> r[U];
@@ -280,9 +283,9 @@ template <typename T>
 __global__ void __launch_bounds__(256) logprob_rows_kernel(Logits L, const RowSum* __restrict__ part, int pieces,
                                                            int lanes, Scale c, double inv_temp,
                                                            float* __restrict__ logp, RowState* __restrict__ rows) {
-  const int64_t row = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+  const unsigned row = blockIdx.x * (256u / lanes) + threadIdx.x / lanes;
   const bool there = row < L.B * L.S;
-  const int64_t b = row / L.S, s = row % L.S, t = there ? L.target_of(b, s) : -1;
+  const int64_t b = L.sequence_of(row), s = L.token_of(row), t = there ? L.target_of(b, s) : -1;
   RowState st{0.f, 0.f, 0.f, 0.f};
   double S, lp = 0.0;
   join_pieces(part, pieces, lanes, row, t >= 0, c, &st.M, &S);
@@ -347,8 +350,8 @@ __global__ void __launch_bounds__(256) policy_rows_kernel(Logits L, const RowSum
                                                           int lanes, Scale c, double inv_temp, PolicyArgs a, int segs,
                                                           float* __restrict__ logp, RowState* __restrict__ rows,
                                                           double4* __restrict__ seg) {
-  const int64_t b = blockIdx.x / segs;
-  const int64_t s = (int64_t)(blockIdx.x % segs) * (256 / lanes) + threadIdx.x / lanes, row = b * L.S + s;
+  const int64_t b = blockIdx.x / (unsigned)segs;
+  const int64_t s = (int64_t)(blockIdx.x % (unsigned)segs) * (256 / lanes) + threadIdx.x / lanes, row = b * L.S + s;
   const int64_t t = s < L.S ? L.target_of(b, s) : -1;
   double v[4] = {0.0, 0.0, 0.0, 0.0};
   RowState st{0.f, 0.f, 0.f, 0.f};
@@ -401,8 +404,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) pair_rows_kernel(Logits L, const RowSum* __restrict__ part, int pieces,
                                                         int lanes, Scale c, int segs, RowState* __restrict__ rows,
                                                         double2* __restrict__ seg) {
-  const int64_t b = blockIdx.x / segs;
-  const int64_t s = (int64_t)(blockIdx.x % segs) * (256 / lanes) + threadIdx.x / lanes, row = b * L.S + s;
+  const int64_t b = blockIdx.x / (unsigned)segs;
+  const int64_t s = (int64_t)(blockIdx.x % (unsigned)segs) * (256 / lanes) + threadIdx.x / lanes, row = b * L.S + s;
   const int64_t t = s < L.S ? L.target_of(b, s) : -1;
   double v[2] = {0.0, 0.0};
   RowState st{0.f, 0.f, 0.f, 0.f};
@@ -506,13 +509,14 @@ __global__ void __launch_bounds__(kGradThreads) logit_grad_kernel(Logits L, Scal
                                                                   float inv_temp, int spans, int64_t units,
                                                                   int unless_one, T* __restrict__ dz) {
   if (unless_one && *gout.p == 1.f) return;
-  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const int64_t row = unit / spans, b = row / L.S, s0 = row % L.S;
-    const int begin = (int)(unit % spans) * kGradSpan<T>, V = (int)L.V, t = (int)L.target_of(b, s0);
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const unsigned unit = (unsigned)u, row = unit / (unsigned)spans;  // (units are below 2^31)
+    const int64_t b = L.sequence_of(row), s0 = L.token_of(row);
+    const int begin = (int)(unit % (unsigned)spans) * kGradSpan<T>, V = (int)L.V, t = (int)L.target_of(b, s0);
     // the lane's logit behind the last whole chunk, where it has one and the span reaches there
     const int last = whole<T>(V) + (int)threadIdx.x;
     const bool tail = last < V && whole<T>(V) - begin < kGradSpan<T> && whole<T>(V) >= begin;
-    T* out = dz + row * L.V;
+    T* out = dz + (int64_t)row * L.V;
     if (t < 0) {
       write_zeros<T, kGradChunks, kGradThreads>(out, begin, V);
       if (tail) out[last] = (T)0.f;
@@ -560,8 +564,9 @@ __global__ void __launch_bounds__(1024) policy_weight_kernel(Logits L, int by_se
     }
   } else {
     int n = 0;
-#pragma unroll 4
-    for (int64_t i = threadIdx.x; i < L.B * L.S; i += 1024) n += L.target_of(i / L.S, i % L.S) >= 0 ? 1 : 0;
+    const unsigned N = (unsigned)(L.B * L.S);
+#pragma unroll 8
+    for (unsigned i = threadIdx.x; i < N; i += 1024) n += L.target_of(L.sequence_of(i), L.token_of(i)) >= 0 ? 1 : 0;
     v[0] = (double)n;
   }
   block_sums64<1, 16>(v);
@@ -604,7 +609,7 @@ __global__ void __launch_bounds__(NT, WAVES) policy_fused_kernel(Logits L, Scale
                                                                  const float* __restrict__ weight,
                                                                  float* __restrict__ logp, RowState* __restrict__ rows,
                                                                  double4* __restrict__ terms, T* __restrict__ dz) {
-  const int64_t row = blockIdx.x, b = row / L.S, s0 = row % L.S;
+  const int64_t row = blockIdx.x, b = L.sequence_of(blockIdx.x), s0 = L.token_of(blockIdx.x);
   const int V = (int)L.V, t = (int)L.target_of(b, s0), last = whole<T>(V) + (int)threadIdx.x;
   T* out = dz + row * L.V;
   if (t < 0) {
@@ -661,7 +666,8 @@ __global__ void __launch_bounds__(1024) policy_sum_kernel(const double4* __restr
                                                           const double* __restrict__ count, float* __restrict__ loss,
                                                           float* __restrict__ stats) {
   double v[3] = {0.0, 0.0, 0.0};
-  for (int64_t i = threadIdx.x; i < N; i += 1024) {
+#pragma unroll 8
+  for (unsigned i = threadIdx.x; i < (unsigned)N; i += 1024) {
     const double4 x = terms[i];
     v[0] += x.x;
     v[1] += x.y;
