@@ -98,6 +98,10 @@ Tensor unit_stride(const Tensor& z) {
   return z.defined() && z.dim() >= 2 && z.size(-1) != 1 && z.stride(-1) != 1 ? z.contiguous() : z;
 }
 
+// Inputs that carry no gradient, whatever they came from
+Tensor fixed(const Tensor& t) { return t.defined() && t.requires_grad() ? t.detach() : t; }
+OptTensor fixed(const OptTensor& t) { return has(t) ? OptTensor(fixed(*t)) : t; }
+
 bool wants_grad(const Tensor& z) { return torch::GradMode::is_enabled() && z.requires_grad(); }
 
 // One allocation of scratch and state: sections of `bytes`, each 256-byte aligned
@@ -297,7 +301,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, con
                                                        double kl_coef, bool by_sequence, int64_t ignore_index,
                                                        double temperature, double scale) {
   const Tensor z = unit_stride(logits);
-  const auto r = PolicyLoss::apply(z, target, old_logp, advantages, ref_logp, clip, clip_high, kl_coef, by_sequence,
+  const auto r = PolicyLoss::apply(z, target, fixed(old_logp), fixed(advantages), fixed(ref_logp), clip, clip_high, kl_coef, by_sequence,
                                    ignore_index, temperature, scale, z.defined() && wants_grad(z));
   return {r[0], r[1], r[2], r[3]};
 }
@@ -305,7 +309,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, con
 std::tuple<Tensor, Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& target,
                                                    const OptTensor& ref_logp, double beta, double smoothing,
                                                    bool average, int64_t ignore_index, double scale) {
-  const auto r = PreferenceLoss::apply(unit_stride(logits), target, ref_logp, beta, smoothing, average, ignore_index,
+  const auto r = PreferenceLoss::apply(unit_stride(logits), target, fixed(ref_logp), beta, smoothing, average, ignore_index,
                                        scale);
   return {r[0], r[1], r[2]};
 }

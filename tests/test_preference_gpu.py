@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from distributed_training_amd.ops import preference
 from tests import preference_oracle as oracle
@@ -362,6 +363,29 @@ def test_captured_and_replayed(shape):
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(out, want))
         del want, new
+
+
+@pytest.mark.parametrize("S", [6, 150])
+def test_under_inference_mode_hooks_and_checkpoints(S):
+    """Scoring under inference_mode, inputs that happen to require a gradient, saved tensors kept on the host, a loss that a
+    checkpoint recomputes: the same bits as the plain call."""
+    z, target, old, ref, adv = _case(4, S, 1003, torch.bfloat16)
+    want = _all_three(z, target, old, ref, adv)
+    with torch.inference_mode():
+        assert torch.equal(preference.token_logprobs(z * 1.0, target), want[0])
+        assert torch.equal(preference.preference_loss(z * 1.0, target).logp, want[8])
+    loose = [t.clone().requires_grad_() for t in (old, ref, adv)]
+    assert not preference.policy_loss(z, target, loose[0], loose[2], loose[1]).loss.requires_grad
+    for x, y in zip(_all_three(z, target, loose[0], loose[1], loose[2]), want):
+        assert torch.equal(x, y)
+    with torch.autograd.graph.save_on_cpu():
+        for x, y in zip(_all_three(z, target, old, ref, adv), want):
+            assert torch.equal(x, y)
+    leaf = z.clone().requires_grad_()
+    loss = torch.utils.checkpoint.checkpoint(
+        lambda x: preference.policy_loss(x * 1.0, target, old, adv, ref, kl_coef=0.1).loss, leaf, use_reentrant=False)
+    loss.backward()
+    assert torch.equal(loss.detach(), want[1]) and torch.equal(leaf.grad, want[6])
 
 
 def test_refusals_on_the_device():
