@@ -18,6 +18,10 @@ int64_t dta_grad_sumsq_parts(const int64_t*, int);
 hipError_t dta_grad_sumsq(void* const*, const int64_t*, const int*, int, double*, int64_t, double*, float*,
                           hipStream_t);
 hipError_t dta_grad_clip(void* const*, const int64_t*, const int*, int, const double*, double, hipStream_t);
+hipError_t dta_grad_clip_norm(void* const*, const int64_t*, const int*, int, double*, int64_t, double*, float*, double,
+                              hipStream_t);
+int dta_grad_is_small(const int64_t*, int);
+hipError_t dta_grad_clip_small(void* const*, const int64_t*, const int*, int, double, float*, hipStream_t);
 
 namespace {
 
@@ -379,10 +383,37 @@ void grad_clip_(const std::vector<Tensor>& grads, const Tensor& sumsq, double ma
   TORCH_CHECK(sumsq.device() == grads[0].device() && sumsq.scalar_type() == torch::kFloat64 && sumsq.numel() == 1,
               "sumsq: f64 scalar on the gradients' GPU");
   const at::DeviceGuard guard(grads[0].device());
+  for (const auto& t : grads) t.unsafeGetTensorImpl()->bump_version();  // (refuses inference tensors)
   ok(dta_grad_clip(g.p.data(), g.numel.data(), g.type.data(), (int)g.p.size(), sumsq.data_ptr<double>(), max_norm,
                    stream_on(grads[0])),
      "grad_clip");
-  for (const auto& t : grads) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// Norm and clip of gradients on one device: the norm (f32 scalar)
+Tensor clip_all(const GradList& g, c10::Device device, double max_norm) {
+  const at::DeviceGuard guard(device);
+  const hipStream_t st = c10::hip::getCurrentHIPStream(device.index()).stream();
+  const int n = (int)g.p.size();
+  Tensor norm = torch::empty({}, torch::TensorOptions().device(device).dtype(torch::kFloat32));
+  if (dta_grad_is_small(g.numel.data(), n)) {
+    ok(dta_grad_clip_small(g.p.data(), g.numel.data(), g.type.data(), n, max_norm, norm.data_ptr<float>(), st),
+       "grad_clip");
+    return norm;
+  }
+  const int64_t parts = dta_grad_sumsq_parts(g.numel.data(), n);
+  Tensor part = torch::empty({parts + 1}, norm.options().dtype(torch::kFloat64));
+  double* scratch = part.data_ptr<double>();
+  ok(dta_grad_clip_norm(g.p.data(), g.numel.data(), g.type.data(), n, scratch + 1, parts, scratch,
+                        norm.data_ptr<float>(), max_norm, st),
+     "grad_clip");
+  return norm;
+}
+
+Tensor clip_grads_(const std::vector<Tensor>& grads, double max_norm) {
+  GradList g = grads_arg(grads);
+  g.drop_repeats();
+  for (const auto& t : grads) t.unsafeGetTensorImpl()->bump_version();  // (refuses inference tensors)
+  return clip_all(g, grads[0].device(), max_norm);
 }
 
 // The whole of clip_grad_norm_ for parameters whose gradients all lie dense on one GPU: the norm, or None where they
@@ -401,14 +432,8 @@ OptTensor clip_params_(const std::vector<Tensor>& params, double max_norm) {
   }
   if (grads.empty()) return c10::nullopt;
   g.drop_repeats();  // a parameter listed twice, or a gradient that two share, counts and is clipped once
-  const at::DeviceGuard guard(grads[0].device());
-  const hipStream_t st = stream_on(grads[0]);
-  const auto sn = sumsq_of(g, grads[0].device(), st);
-  ok(dta_grad_clip(g.p.data(), g.numel.data(), g.type.data(), (int)g.p.size(), std::get<0>(sn).data_ptr<double>(),
-                   max_norm, st),
-     "grad_clip");
-  for (const auto& t : grads) t.unsafeGetTensorImpl()->bump_version();
-  return std::get<1>(sn);
+  for (const auto& t : grads) t.unsafeGetTensorImpl()->bump_version();  // (refuses inference tensors)
+  return clip_all(g, grads[0].device(), max_norm);
 }
 
 }  // namespace
@@ -424,5 +449,6 @@ void dta_register_pref(pybind11::module_& m) {
         py::arg("beta"), py::arg("smoothing"), py::arg("average"), py::arg("ignore_index"), py::arg("scale"));
   m.def("grad_sumsq", &grad_sumsq, py::arg("grads"));
   m.def("grad_clip_", &grad_clip_, py::arg("grads"), py::arg("sumsq"), py::arg("max_norm"));
+  m.def("clip_grads_", &clip_grads_, py::arg("grads"), py::arg("max_norm"));
   m.def("clip_params_", &clip_params_, py::arg("params"), py::arg("max_norm"));
 }

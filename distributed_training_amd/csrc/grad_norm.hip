@@ -74,9 +74,19 @@ __device__ __forceinline__ double sumsq_unit(const T* __restrict__ p, int64_t c0
           acc = fma(d, d, acc);
         }
     }
-  } else {
-    for (int64_t i = c0 + threadIdx.x; i < numel; i += 256) {
-      const double d = (double)p[i];
+  } else {  // a tensor's end: whole vectors, then up to W - 1 elements
+    const int64_t end = numel - (numel - c0) % W;
+#pragma unroll 4
+    for (int64_t i = c0 + threadIdx.x * W; i < end; i += STEP) {
+      const typename Pack<T>::V v = load_v<false, typename Pack<T>::V>(p + i);
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const double d = (double)v[j];
+        acc = fma(d, d, acc);
+      }
+    }
+    if (end + threadIdx.x < numel) {
+      const double d = (double)p[end + threadIdx.x];
       acc = fma(d, d, acc);
     }
   }
@@ -85,13 +95,13 @@ __device__ __forceinline__ double sumsq_unit(const T* __restrict__ p, int64_t c0
 
 // The coefficient is used in fp32 (2^-24 relative; fp64 gradients take it whole) and each product rounded to T
 template <typename T>
+__device__ __forceinline__ T scaled(T x, double coef) {
+  if constexpr (sizeof(T) == 8) return x * coef;
+  else return (T)((float)x * (float)coef);
+}
+template <typename T>
 __device__ __forceinline__ void scale_unit(T* __restrict__ p, int64_t c0, int64_t numel, double coef) {
   constexpr int W = Pack<T>::n, STEP = 256 * W, LOADS = kUnit / STEP, U = LOADS < 4 ? LOADS : 4;
-  const float cf = (float)coef;
-  auto mul = [&](T x) -> T {
-    if constexpr (sizeof(T) == 8) return x * coef;
-    else return (T)((float)x * cf);
-  };
   if (c0 + kUnit <= numel) {
     for (int l = 0; l < LOADS; l += U) {
       typename Pack<T>::V v[U];
@@ -101,14 +111,33 @@ __device__ __forceinline__ void scale_unit(T* __restrict__ p, int64_t c0, int64_
 #pragma unroll
       for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) v[u][j] = mul(v[u][j]);
+        for (int j = 0; j < W; ++j) v[u][j] = scaled<T>(v[u][j], coef);
         __builtin_nontemporal_store(
             v[u], reinterpret_cast<typename Pack<T>::V*>(p + c0 + (l + u) * STEP + threadIdx.x * W));
       }
     }
   } else {
-    for (int64_t i = c0 + threadIdx.x; i < numel; i += 256) p[i] = mul(p[i]);
+    const int64_t end = numel - (numel - c0) % W;
+#pragma unroll 4
+    for (int64_t i = c0 + threadIdx.x * W; i < end; i += STEP) {
+      typename Pack<T>::V v = load_v<false, typename Pack<T>::V>(p + i);
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[j] = scaled<T>(v[j], coef);
+      *reinterpret_cast<typename Pack<T>::V*>(p + i) = v;
+    }
+    if (end + threadIdx.x < numel) p[end + threadIdx.x] = scaled<T>(p[end + threadIdx.x], coef);
   }
+}
+
+// The tensor that unit u belongs to: the last one that starts at or before it
+__device__ __forceinline__ int tensor_of(const NormJobs& jobs, int u) {
+  int lo = 0, hi = jobs.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (jobs.start[mid] <= u) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
 }
 
 // This workgroup's run of units, from its end to its start where BACK: f(pointer, type, first element, numel, whether
@@ -118,14 +147,7 @@ __device__ __forceinline__ void walk_units(const NormJobs& jobs, F f) {
   const int u0 = (int)((int64_t)jobs.units * blockIdx.x / gridDim.x);
   const int u1 = (int)((int64_t)jobs.units * (blockIdx.x + 1) / gridDim.x);
   if (u0 >= u1) return;
-  const int first = BACK ? u1 - 1 : u0;
-  int lo = 0, hi = jobs.n - 1;  // the last tensor that starts at or before the first unit
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (jobs.start[mid] <= first) lo = mid;
-    else hi = mid - 1;
-  }
-  int j = lo;
+  int j = tensor_of(jobs, BACK ? u1 - 1 : u0);
   for (int i = 0; i < u1 - u0; ++i) {
     const int u = BACK ? u1 - 1 - i : u0 + i;
     if (BACK) while (u < jobs.start[j]) --j;
@@ -184,9 +206,8 @@ __global__ void __launch_bounds__(1024) grad_norm_kernel(const double* __restric
 
 // A norm within the bound leaves every gradient as it is: the workgroups end without touching them.  A NaN norm
 // gives a NaN coefficient (not 1), an infinite one 0, as min(1, max_norm / (norm + 1e-6)) says.
-__global__ void __launch_bounds__(256) grad_clip_kernel(NormJobs jobs, const double* __restrict__ sumsq,
-                                                        double max_norm) {
-  const double coef = max_norm / (sqrt(*sumsq) + 1e-6);
+__device__ __forceinline__ void clip_units(const NormJobs& jobs, double root, double max_norm) {
+  const double coef = max_norm / (root + 1e-6);
   if (coef >= 1.0) return;
   walk_units<true>(jobs, [&](void* p, int type, int64_t c0, int64_t numel, bool) {
     if (type == 1) scale_unit((bf16*)p, c0, numel, coef);
@@ -195,9 +216,80 @@ __global__ void __launch_bounds__(256) grad_clip_kernel(NormJobs jobs, const dou
     else scale_unit((double*)p, c0, numel, coef);
   });
 }
+__global__ void __launch_bounds__(256) grad_clip_kernel(NormJobs jobs, const double* __restrict__ sumsq,
+                                                        double max_norm) {
+  clip_units(jobs, sqrt(*sumsq), max_norm);
+}
+// For few partial sums: every workgroup adds them up itself, which spares the launch of grad_norm_kernel.  A pass in us,
+// two launches / three: 30 K fp32 elements in 40 tensors 14.3 / 19.5, 2 M in 4 tensors 11.1 / 15.1, 8 M (977 partial
+// sums) 15.2 / 16.4; the read of the sums grows with the square of their number, so it stops there.
+constexpr int kJoined = 1024;
+__global__ void __launch_bounds__(256) grad_clip_joined_kernel(NormJobs jobs, const double* __restrict__ part, int n,
+                                                               float* __restrict__ norm, double max_norm) {
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < n; i += 256) acc += part[i];
+  const double root = sqrt(block_sum64<256>(acc));
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)root;
+  clip_units(jobs, root, max_norm);
+}
 
-// The launches' tables for `count` tensors
-static std::vector<NormJobs> tables(void* const* p, const int64_t* numel, const int* type, int count) {
+// Norm and clip of a small model in one launch of one workgroup (a wave a unit of kSmallUnit elements): the other forms
+// are mostly launches there.  A pass in us, one launch / two: 100 elements 4.5 / 10.7, 11 K in 4 tensors (23 units)
+// 7.3 / 10.7, 4 K in 64 tensors (64 units) 11.9 / 15.9, 32 K in 4 tensors (64 units) 13.1 / 11.1, or 7.6 / 10.9 where the
+// norm is within the bound.
+constexpr int kSmallUnit = 512, kSmallUnits = 64;
+
+template <typename T>
+__device__ __forceinline__ double small_sumsq(const T* p, int64_t c0, int64_t numel) {
+  double acc = 0.0;
+#pragma unroll
+  for (int k = 0; k < kSmallUnit / 64; ++k) {
+    const int64_t i = c0 + k * 64 + (threadIdx.x & 63);
+    const double d = i < numel ? (double)p[i] : 0.0;
+    acc = fma(d, d, acc);
+  }
+  return acc;
+}
+template <typename T>
+__device__ __forceinline__ void small_scale(T* p, int64_t c0, int64_t numel, double coef) {
+#pragma unroll
+  for (int k = 0; k < kSmallUnit / 64; ++k) {
+    const int64_t i = c0 + k * 64 + (threadIdx.x & 63);
+    if (i < numel) p[i] = scaled<T>(p[i], coef);
+  }
+}
+
+__global__ void __launch_bounds__(1024) grad_clip_small_kernel(NormJobs jobs, double max_norm,
+                                                               float* __restrict__ norm) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  auto walk = [&](auto f) {
+    for (int u = wave; u < jobs.units; u += 16) {
+      const int j = tensor_of(jobs, u);
+      f(jobs.p[j], (int)(jobs.numel_type[j] & 3), (int64_t)(u - jobs.start[j]) * kSmallUnit, jobs.numel_type[j] >> 2);
+    }
+  };
+  double acc = 0.0;
+  walk([&](void* p, int type, int64_t c0, int64_t numel) {
+    if (type == 1) acc += small_sumsq((const bf16*)p, c0, numel);
+    else if (type == 0) acc += small_sumsq((const float*)p, c0, numel);
+    else if (type == 2) acc += small_sumsq((const _Float16*)p, c0, numel);
+    else acc += small_sumsq((const double*)p, c0, numel);
+  });
+  const double root = sqrt(block_sum64<1024>(acc));
+  if (threadIdx.x == 0) *norm = (float)root;
+  const double coef = max_norm / (root + 1e-6);
+  if (coef >= 1.0) return;
+  walk([&](void* p, int type, int64_t c0, int64_t numel) {
+    if (type == 1) small_scale((bf16*)p, c0, numel, coef);
+    else if (type == 0) small_scale((float*)p, c0, numel, coef);
+    else if (type == 2) small_scale((_Float16*)p, c0, numel, coef);
+    else small_scale((double*)p, c0, numel, coef);
+  });
+}
+
+// The launches' tables for `count` tensors, in units of kUnit elements
+static std::vector<NormJobs> tables(void* const* p, const int64_t* numel, const int* type, int count,
+                                    int64_t unit = kUnit) {
   constexpr int64_t kMostUnits = 1 << 30;
   std::vector<NormJobs> all;
   int i = 0;
@@ -208,10 +300,10 @@ static std::vector<NormJobs> tables(void* const* p, const int64_t* numel, const 
     int64_t units = 0, bytes = 0;
     int n = 0;
     while (i < count && n < kJobs && units < kMostUnits) {
-      const int64_t left = numel[i] - done, need = (left + kUnit - 1) / kUnit;
+      const int64_t left = numel[i] - done, need = (left + unit - 1) / unit;
       const int64_t take = need < kMostUnits - units ? need : kMostUnits - units;
       if (take > 0) {
-        const int64_t elems = take == need ? left : take * kUnit;
+        const int64_t elems = take == need ? left : take * unit;
         const int size = type[i] == 0 ? 4 : type[i] == 3 ? 8 : 2;
         jobs.p[n] = static_cast<char*>(p[i]) + done * size;
         jobs.numel_type[n] = elems * 4 + type[i];
@@ -248,27 +340,70 @@ int64_t dta_grad_sumsq_parts(const int64_t* numel, int count) {
   return (count / kJobs + 2 * (units >> 30) + 1) * (units < kNormGrid ? units + 1 : kNormGrid);
 }
 
-// sumsq (1 double), norm (1 float); part: dta_grad_sumsq_parts doubles of scratch
-hipError_t dta_grad_sumsq(void* const* p, const int64_t* numel, const int* type, int count, double* part,
-                          int64_t parts, double* sumsq, float* norm, hipStream_t st) {
-  int64_t used = 0;
-  for (const NormJobs& jobs : tables(p, numel, type, count)) {
+static hipError_t partial_sums(const std::vector<NormJobs>& all, double* part, int64_t parts, int* used,
+                               hipStream_t st) {
+  *used = 0;
+  for (const NormJobs& jobs : all) {
     const int grid = workgroups(jobs);
-    if (used + grid > parts) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(grad_sumsq_kernel, dim3(grid), dim3(256), 0, st, jobs, part + used);
+    if (*used + grid > parts) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(grad_sumsq_kernel, dim3(grid), dim3(256), 0, st, jobs, part + *used);
     DTA_HIP_CHECK(hipGetLastError());
-    used += grid;
+    *used += grid;
   }
-  hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(1024), 0, st, part, (int)used, sumsq, norm);
-  return hipGetLastError();
+  return hipSuccess;
 }
-
-hipError_t dta_grad_clip(void* const* p, const int64_t* numel, const int* type, int count, const double* sumsq,
-                         double max_norm, hipStream_t st) {
-  const std::vector<NormJobs> all = tables(p, numel, type, count);
+static hipError_t clip_by(const std::vector<NormJobs>& all, const double* sumsq, double max_norm, hipStream_t st) {
   for (size_t i = all.size(); i-- > 0;) {  // the last launch's gradients are the ones that are still cached
     hipLaunchKernelGGL(grad_clip_kernel, dim3(workgroups(all[i])), dim3(256), 0, st, all[i], sumsq, max_norm);
     DTA_HIP_CHECK(hipGetLastError());
   }
   return hipSuccess;
+}
+
+// sumsq (1 double), norm (1 float); part: dta_grad_sumsq_parts doubles of scratch
+hipError_t dta_grad_sumsq(void* const* p, const int64_t* numel, const int* type, int count, double* part,
+                          int64_t parts, double* sumsq, float* norm, hipStream_t st) {
+  int used;
+  DTA_HIP_CHECK(partial_sums(tables(p, numel, type, count), part, parts, &used, st));
+  hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(1024), 0, st, part, used, sumsq, norm);
+  return hipGetLastError();
+}
+
+hipError_t dta_grad_clip(void* const* p, const int64_t* numel, const int* type, int count, const double* sumsq,
+                         double max_norm, hipStream_t st) {
+  return clip_by(tables(p, numel, type, count), sumsq, max_norm, st);
+}
+
+// dta_grad_sumsq and dta_grad_clip in one
+hipError_t dta_grad_clip_norm(void* const* p, const int64_t* numel, const int* type, int count, double* part,
+                              int64_t parts, double* sumsq, float* norm, double max_norm, hipStream_t st) {
+  const std::vector<NormJobs> all = tables(p, numel, type, count);
+  int used;
+  DTA_HIP_CHECK(partial_sums(all, part, parts, &used, st));
+  if (all.size() == 1 && used <= kJoined) {
+    hipLaunchKernelGGL(grad_clip_joined_kernel, dim3(workgroups(all[0])), dim3(256), 0, st, all[0], part, used, norm,
+                       max_norm);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(1024), 0, st, part, used, sumsq, norm);
+  DTA_HIP_CHECK(hipGetLastError());
+  return clip_by(all, sumsq, max_norm, st);
+}
+
+// Whether the gradients are few enough for dta_grad_clip_small
+int dta_grad_is_small(const int64_t* numel, int count) {
+  int64_t units = 0;
+  if (count > kJobs) return 0;
+  for (int i = 0; i < count && units <= kSmallUnits; ++i) units += (numel[i] + kSmallUnit - 1) / kSmallUnit;
+  return units <= kSmallUnits;
+}
+
+// dta_grad_clip_norm in one launch
+hipError_t dta_grad_clip_small(void* const* p, const int64_t* numel, const int* type, int count, double max_norm,
+                               float* norm, hipStream_t st) {
+  if (!dta_grad_is_small(numel, count)) return hipErrorInvalidValue;
+  const std::vector<NormJobs> all = tables(p, numel, type, count, kSmallUnit);
+  NormJobs none{};
+  hipLaunchKernelGGL(grad_clip_small_kernel, dim3(1), dim3(1024), 0, st, all.empty() ? none : all[0], max_norm, norm);
+  return hipGetLastError();
 }

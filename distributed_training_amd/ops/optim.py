@@ -75,11 +75,15 @@ def grad_sumsq(tensors: Iterable[torch.Tensor]) -> Tuple[torch.Tensor, torch.Ten
     return first, norm
 
 
+def _check_max_norm(max_norm: float) -> None:
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative (got {max_norm})")
+
+
 def grad_clip_(tensors: Iterable[torch.Tensor], sumsq: torch.Tensor, max_norm: float) -> None:
     """Every tensor times ``min(1, max_norm / (sqrt(sumsq) + 1e-6))`` in place; ``sumsq``: the 0-dim fp64 tensor of
     :func:`grad_sumsq`, summed over ranks where the gradients are sharded.  Within the bound nothing is touched."""
-    if not max_norm >= 0.0:
-        raise ValueError(f"max_norm must not be negative (got {max_norm})")
+    _check_max_norm(max_norm)
     for device, ts in _by_device(tensors).items():
         if device.type != "cuda":
             coef = (float(max_norm) / (sumsq.to(device).sqrt() + 1e-6)).clamp(max=1.0)
@@ -100,6 +104,22 @@ def global_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]]) -> torch.T
 
 
 @torch.no_grad()
+def clip_grads_(tensors: Iterable[torch.Tensor], max_norm: float) -> torch.Tensor:
+    """:func:`clip_grad_norm_` for the gradients themselves (each listed once): scaled in place, their global
+    norm returned."""
+    _check_max_norm(max_norm)
+    devices = _by_device(tensors)
+    if len(devices) == 1:
+        ((device, ts),) = devices.items()
+        if device.type == "cuda" and all(_fills_memory(t) for t in ts):
+            return native().clip_grads_(ts, float(max_norm))
+    grads = [t for ts in devices.values() for t in ts]
+    sumsq, norm = grad_sumsq(grads)
+    grad_clip_(grads, sumsq, max_norm)
+    return norm
+
+
+@torch.no_grad()
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scale the parameters' gradients in place so that their global 2-norm is at most ``max_norm``, and return the
@@ -109,8 +129,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     norm is within the bound: no host sync unless ``error_if_nonfinite`` asks for one.
 
     Gradients held by a DDP / FSDP engine: call the engine's own ``clip_grad_norm_``, which also sums over shards."""
-    if not max_norm >= 0.0:
-        raise ValueError(f"max_norm must not be negative (got {max_norm})")
+    _check_max_norm(max_norm)
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     if not error_if_nonfinite and params and params[0].is_cuda:
         norm = native().clip_params_(params, float(max_norm))  # one call for gradients that lie dense on one GPU
@@ -124,8 +143,10 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     grads = list(seen.values())
     if not grads:
         return torch.zeros(())
+    if not error_if_nonfinite:
+        return clip_grads_(grads, max_norm)
     sumsq, norm = grad_sumsq(grads)
-    if error_if_nonfinite and not bool(torch.isfinite(norm)):
+    if not bool(torch.isfinite(norm)):
         raise RuntimeError(f"the global gradient norm is {float(norm)}, so the gradients cannot be clipped")
     grad_clip_(grads, sumsq, max_norm)
     return norm

@@ -210,22 +210,22 @@ def clip_flat_grad_norm_(fg: FlatParamGroup, max_norm: float, comm: Any = None, 
     does not change the norm.  Returns the total norm (0-dim tensor)."""
     if not fg.prepare_grads_for_step():
         return torch.zeros((), device=fg.grad.device)
-    from ..ops.optim import grad_clip_, grad_sumsq
+    from ..ops.optim import clip_grads_, grad_clip_, grad_sumsq
 
     g = fg.grad
-    sq64, norm = grad_sumsq([g])
-    if sharded and comm is not None and comm.world_size > 1:
-        sq = sq64.float().reshape(1)
-        dev = getattr(comm, "device", None)
-        if dev is not None and sq.device != torch.device(dev):  # host-resident shards, device communicator
-            sq_d = sq.to(dev)
-            comm.all_reduce(sq_d, op="sum")
-            sq = sq_d.to(sq.device)
-        else:
-            comm.all_reduce(sq, op="sum")
-        sq64, norm = sq.double(), sq.sqrt()
-    grad_clip_([g], sq64, max_norm)
-    return norm.reshape(())
+    if not (sharded and comm is not None and comm.world_size > 1):
+        return clip_grads_([g], max_norm).reshape(())
+    sq = grad_sumsq([g])[0].float().reshape(1)
+    dev = getattr(comm, "device", None)
+    if dev is not None and sq.device != torch.device(dev):  # host-resident shards, device communicator
+        sq_d = sq.to(dev)
+        comm.all_reduce(sq_d, op="sum")
+        sq = sq_d.to(sq.device)
+    else:
+        comm.all_reduce(sq, op="sum")
+    sq = sq.reshape(())
+    grad_clip_([g], sq.double(), max_norm)
+    return sq.sqrt()
 
 
 def plan_buckets(numels: Sequence[int], esize: int, cap_bytes: int, first_cap_bytes: int) -> List[List[int]]:

@@ -63,6 +63,18 @@ def test_many_tensors_of_mixed_types(count):
     _check(_params(sizes, TYPES, seed=count, offset=1), 1.0)
 
 
+@pytest.mark.parametrize("sizes", [[20 * 512, 512, 512, 1], [1] * 64, [0, 513, 0, 64 * 512 - 1024], [1] * 65, [32769],
+                                   [7] * 161, [64] * 64, [1024 * 8192], [1024 * 8192 - 5, 9]])
+def test_small_models(sizes):
+    """Up to 64 units of 512 elements: one launch; up to 1024 of 8192 in at most 160 tensors: two.  The sizes around."""
+    for dtypes in ([torch.float32], TYPES):
+        for max_norm in (0.2, 1e6):
+            _check(_params(sizes, dtypes, seed=len(sizes), offset=1), max_norm)
+    q = torch.nn.Parameter(torch.empty(0, device=DEV))
+    q.grad = torch.empty(0, device=DEV)
+    assert float(optim.clip_grad_norm_([q], 1.0)) == 0.0
+
+
 def test_within_the_bound_nothing_changes():
     _check(_params([1000, 3], [torch.bfloat16, torch.float32]), 1e6)
     params = _params([3000], [torch.float32])
