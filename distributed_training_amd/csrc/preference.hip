@@ -737,10 +737,11 @@ static TokenArray array_of(const PrefTokens& t) { return {t.p, t.sb, t.ss}; }
     default: return hipErrorInvalidValue;             \
   }
 
-// Workgroups of the passes over the logits have to fit a launch
+// A launch takes fewer than 2^32 threads, and the row passes give a row a workgroup of 256; units are counted in 32 bits
+constexpr int64_t kMostGroups = ((int64_t)1 << 24) - 1;
 int dta_pref_fits(int64_t N, int64_t V) {
-  const int64_t most = (int64_t)1 << 31, spans = (V + kGradSpan<float> - 1) / kGradSpan<float>;
-  return N >= 0 && V > 0 && N < most && V < ((int64_t)1 << 28) && N * spans < most;
+  const int64_t spans = (V + kGradSpan<float> - 1) / kGradSpan<float>;
+  return N >= 0 && V > 0 && N <= kMostGroups && V < ((int64_t)1 << 28) && N * spans < ((int64_t)1 << 31);
 }
 int64_t dta_pref_parts(int64_t N, int64_t V) { return N * lse_shape(N, V).pieces; }
 int64_t dta_pref_segs(int64_t B, int64_t S, int64_t V) { return B * segments(S, lse_shape(B * S, V)); }
@@ -790,7 +791,7 @@ hipError_t dta_pref_policy(const PrefLogits& l, int type, double temperature, co
 // several: 64 rows of 50304 18.2 / 17.8, of 128256 26.7 / 22.4; 128 rows 18.4 / 21.2 and 27.5 / 30.9; 2048 rows 85 / 110
 // and 202 / 258.
 int dta_pref_policy_fused(int type, int64_t N, int64_t V) {
-  return N >= 128 && V <= (type == 0 ? 65536 : 131072);
+  return N >= 128 && N < (1 << 22) && V <= (type == 0 ? 65536 : 131072);  // (workgroups of up to 1024 threads)
 }
 
 template <typename T, int NT, int CHUNKS, int WAVES>
@@ -869,7 +870,7 @@ hipError_t dta_pref_grad(const PrefLogits& l, int type, double temperature, cons
     const int spans = (int)((L.V + kGradSpan<T> - 1) / kGradSpan<T>);
     const int64_t units = N * spans;
     // (a launch that is expected to end at once is a small one, whose workgroups walk over the rows if they have to)
-    const int64_t grid = unless_one ? min(units, (int64_t)2048) : units;
+    const int64_t grid = min(units, unless_one ? (int64_t)2048 : kMostGroups);
     hipLaunchKernelGGL(logit_grad_kernel<T>, dim3((unsigned)grid), dim3(kGradThreads), 0, st, L, scale_of(temperature),
                        (const RowState*)rows, weight, array_of(gout), (float)(1.0 / temperature), spans, units,
                        unless_one, (T*)dz);

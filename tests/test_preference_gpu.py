@@ -402,6 +402,32 @@ def test_refusals_on_the_device():
         preference.preference_loss(z, target, torch.zeros(2))
 
 
+def test_many_rows_of_a_tiny_vocabulary():
+    """The passes take up to 2^24 - 1 rows, the one-pass policy loss up to 2^22 - 1; one more is refused, or done in several
+    passes."""
+    N = 2 ** 24
+    z = torch.zeros(N, 2, device=DEV, dtype=torch.bfloat16)
+    z[:, 1] = 1.0
+    target = torch.ones(N, dtype=torch.int64, device=DEV)
+    with pytest.raises(ValueError, match="too many rows"):
+        preference.token_logprobs(z, target)
+    z = z[:-1].requires_grad_()
+    lp = preference.token_logprobs(z, target[:-1])
+    want = -math.log1p(math.exp(-1.0))
+    assert float((lp.detach() - want).abs().max()) < 1e-6
+    (g,) = torch.autograd.grad(lp.sum(), z)
+    assert float((g.double() - torch.tensor([-1.0, 1.0], device=DEV) * (1 - math.exp(want))).abs().max()) < 2 ** -10
+    for n in (2 ** 22 - 1, 2 ** 22):
+        x = z.detach()[:n].requires_grad_()
+        old, adv = torch.full((n,), want, device=DEV), torch.ones(n, device=DEV)
+        out = preference.policy_loss(x, target[:n], old, adv)
+        assert abs(float(out.loss) + 1.0) < 1e-6 and float(out.clip_fraction) == 0.0
+        out.loss.backward()
+        # k = -1 / n times [-(1 - p), 1 - p], rounded to bf16
+        slope = (1 - math.exp(want)) / n
+        assert float((x.grad.double() - torch.tensor([slope, -slope], device=DEV, dtype=torch.float64)).abs().max()) <= slope * 2 ** -7
+
+
 def test_a_preference_step_end_to_end():
     """A reference model scores, the policy under the DDP engine is trained on pairs and on rewards, gradients are
     clipped, the optimizer steps: the run of operators as a training program has them, its gradients against the same
