@@ -9,7 +9,8 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
-#include <unordered_set>
+#include <algorithm>
+#include <functional>
 #include <vector>
 
 #include "preference.h"
@@ -328,13 +329,30 @@ struct GradList {
     numel.push_back(t.numel());
     type.push_back(type_);
   }
+  int64_t bytes(size_t i) const { return numel[i] * (type[i] == 0 ? 4 : type[i] == 3 ? 8 : 2); }
   // Memory that is listed twice is kept once (two parameters may share a gradient): scaled twice it would depend on
-  // which workgroup comes first
+  // which workgroup comes first.  Gradients that share a part are refused for the same reason.
   void drop_repeats() {
-    std::unordered_set<const void*> seen;
+    std::vector<size_t> order;
+    for (size_t i = 0; i < p.size(); ++i)
+      if (numel[i] > 0) order.push_back(i);
+    std::sort(order.begin(), order.end(), [&](size_t a, size_t b) { return std::less<void*>()(p[a], p[b]); });
+    bool any = false;
+    for (size_t k = 1, last = 0; k < order.size(); ++k) {
+      const size_t i = order[k], j = order[last];
+      if (p[i] == p[j] && numel[i] == numel[j] && type[i] == type[j]) {
+        numel[i] = 0;
+        any = true;
+        continue;
+      }
+      TORCH_CHECK_VALUE(static_cast<char*>(p[j]) + bytes(j) <= static_cast<char*>(p[i]),
+                        "gradients overlap in memory without being the same");
+      last = k;
+    }
+    if (!any) return;
     size_t n = 0;
     for (size_t i = 0; i < p.size(); ++i) {
-      if (numel[i] > 0 && !seen.insert(p[i]).second) continue;
+      if (numel[i] == 0) continue;
       p[n] = p[i];
       numel[n] = numel[i];
       type[n++] = type[i];

@@ -125,8 +125,10 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     """Scale the parameters' gradients in place so that their global 2-norm is at most ``max_norm``, and return the
     norm before (a 0-dim fp32 tensor).  As ``torch.nn.utils.clip_grad_norm_`` with its 2-norm: the coefficient is
     ``min(1, max_norm / (norm + 1e-6))``, a NaN norm makes every gradient NaN; parameters without a gradient are
-    skipped, and one that is listed twice (or a gradient that two share) counts and is scaled once.  On the GPU the norm is one pass over every gradient and the scaling another, left out on the device where the
-    norm is within the bound: no host sync unless ``error_if_nonfinite`` asks for one.
+    skipped, and one that is listed twice (or a gradient that two share) counts and is scaled once; gradients on the
+    GPU that share a part of their memory are refused.  On the GPU the norm is one pass over every gradient and the
+    scaling another, left out on the device where the norm is within the bound: no host sync unless
+    ``error_if_nonfinite`` asks for one.
 
     Gradients held by a DDP / FSDP engine: call the engine's own ``clip_grad_norm_``, which also sums over shards."""
     _check_max_norm(max_norm)
@@ -138,8 +140,12 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     seen: Dict[Any, torch.Tensor] = {}
     for p in params:
         if p.grad is not None:
-            key = (p.grad.data_ptr(), p.grad.device) if p.grad.numel() and p.grad.layout == torch.strided else id(p)
-            seen.setdefault(key, p.grad)
+            g = p.grad
+            key: Any = id(g)
+            if g.layout == torch.strided and g.numel():
+                lies = g.numel() if _fills_memory(g) else (g.shape, g.stride())
+                key = (g.data_ptr(), g.device, g.dtype, lies)
+            seen.setdefault(key, g)
     grads = list(seen.values())
     if not grads:
         return torch.zeros(())

@@ -115,6 +115,24 @@ def test_what_is_listed_twice_is_clipped_once():
     assert ((p.grad.double() - want).abs() <= want.abs() * 1e-5).all()
 
 
+def test_gradients_that_share_a_part_are_refused():
+    base = torch.ones(100, device=DEV)
+    p, q = (torch.nn.Parameter(torch.zeros(n, device=DEV)) for n in (10, 100))
+    for first in (base[:10], base[40:50], base[90:]):
+        p.grad, q.grad = first, base
+        for params in ([p, q], [q, p], [p, p, q]):
+            with pytest.raises(ValueError, match="overlap"):
+                optim.clip_grad_norm_(params, 0.5)
+    assert torch.equal(base, torch.ones_like(base))
+    r = torch.nn.Parameter(torch.zeros(90, device=DEV))
+    p.grad, r.grad = base[:10], base[10:]  # (neighbours in memory are two gradients)
+    assert abs(float(optim.clip_grad_norm_([r, p, r], 11.0)) - 10.0) < 1e-5
+    square = torch.nn.Parameter(torch.zeros(10, 10, device=DEV))
+    square.grad, q.grad = base.view(10, 10).t(), base.view(100)
+    for flag in (False, True):  # one memory in two orders
+        assert abs(float(optim.clip_grad_norm_([square, q], 11.0, error_if_nonfinite=flag)) - 10.0) < 1e-5
+
+
 def test_extremes_and_nonfinite():
     assert abs(float(optim.global_norm(torch.full((10000,), 1e25, device=DEV))) / 1e27 - 1) < 1e-6
     assert abs(float(optim.global_norm(torch.full((10000,), 1e-30, device=DEV))) / 1e-28 - 1) < 1e-6
