@@ -194,14 +194,14 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     const bool fused = grad && dta_pref_policy_fused(type, N, l.V);
     Arena a;
     const int64_t rows = a.add(16 * N), weight = a.add(4 * l.B);
-    const int64_t part = a.add(fused ? 32 * N + 8 : 16 * dta_pref_parts(N, l.V));
+    const int64_t part = a.add(fused ? 16 * N + 8 : 16 * dta_pref_parts(N, l.V));
     const int64_t seg = a.add(fused ? 0 : 32 * dta_pref_segs(l.B, l.S, l.V));
     a.make(z);
     const auto f32 = z.options().dtype(torch::kFloat32);
     Tensor loss = torch::empty({}, f32), stats = torch::empty({2}, f32), logp = torch::empty(target.sizes(), f32);
     if (fused) {
       Tensor dz = torch::empty(z.sizes(), z.options());
-      ok(dta_pref_policy_grad(l, type, temperature, p, reinterpret_cast<double*>(a.at(part)), loss.data_ptr<float>(),
+      ok(dta_pref_policy_grad(l, type, temperature, p, a.at(part), loss.data_ptr<float>(),
                               stats.data_ptr<float>(), logp.data_ptr<float>(), a.at(rows),
                               reinterpret_cast<float*>(a.at(weight)), dz.data_ptr(), st),
          "policy_loss");

@@ -127,6 +127,17 @@ struct RowState {
   float M, l2s, coef, pad;  // coef: dloss/dlp without the sequence's weight
 };
 
+// A row is one workgroup's, or, where it is short (NT = 64), one wave's: four rows in a workgroup of 256 threads, which
+// share nothing and wait for nothing.  A short row in a workgroup of its own left most lanes idle and was bound by the
+// rate at which workgroups start.
+template <int NT> constexpr int kRows = NT == 64 ? 4 : 1;
+template <int NT>
+__device__ __forceinline__ int thread_of() { return NT == 64 ? (int)threadIdx.x & 63 : (int)threadIdx.x; }
+template <int NT>
+__device__ __forceinline__ unsigned group_of() {  // among all groups of NT threads
+  return NT == 64 ? blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
+}
+
 constexpr int kLseThreads = 256;
 
 template <int CTRL, int ROWMASK>
@@ -151,9 +162,14 @@ struct RowSum {  // of a row or a piece of one
   float M, pad;
 };
 
-// A workgroup's threads together
+// A row's threads together
 template <int NW>
 __device__ __forceinline__ RowSum block_join(float m, float s, const Scale& c) {
+  if constexpr (NW == 1) {
+    const float wm = wave_max(m);
+    const double ws = wave_sum64_last((double)(s * c.of_exp(m - (wm == -INFINITY ? 0.f : wm))));
+    return {__shfl(ws, 63, kWave), wm, 0.f};
+  }
   __shared__ float sm[NW];
   __shared__ double sv[NW];
   const float wm = wave_max(m);
@@ -174,20 +190,42 @@ __device__ __forceinline__ RowSum block_join(float m, float s, const Scale& c) {
 }
 
 // ------------------------------------------------------------------ (M, s) of every row
-// Workgroup row * pieces + i: piece i of the row, [i * span, (i + 1) * span).  U chunks a thread are requested before
-// any is used and share one rescaling of the running sum.  Bound by the read: 6.6 TB/s at 8192 x 50304 bf16 (124 us), 6.7
-// at 1999 x 128256 fp32 (152 us).
-template <typename T>
+// Log-probability of the token with logit zt from its row's (M, S), in fp64; a row of nothing but -inf, or with a NaN or
+// +inf, gives NaN.
+__device__ __forceinline__ double row_logprob(float zt, float M, double S, double inv_temp, float* l2s) {
+  const double l2 = log2(S);
+  *l2s = (float)l2;
+  return ((double)zt - (double)M) * inv_temp - l2 * 0.69314718055994530942;
+}
+
+// Group row * pieces + i: piece i of the row, [i * span, (i + 1) * span).  U chunks a thread are requested before
+// any is used and share one rescaling of the running sum.  Bound by the read: 6.7 TB/s at 8192 x 50304 bf16 (123 us), 6.7
+// at 1999 x 128256 fp32 (153 us).
+// LOGPROB (rows of one piece): the row's log-probability and state as well, which spares logprob_rows_kernel.
+template <typename T, int NT, bool LOGPROB>
 __global__ void __launch_bounds__(kLseThreads) lse_partial_kernel(Logits L, Scale c, int pieces, int span,
-                                                                  RowSum* __restrict__ part) {
-  constexpr int NW = kLseThreads / 64, U = 4, W = Chunk<T>::W, STEP = kLseThreads * W;
-  const unsigned row = blockIdx.x / (unsigned)pieces;
+                                                                  RowSum* __restrict__ part, double inv_temp,
+                                                                  float* __restrict__ logp,
+                                                                  RowState* __restrict__ rows) {
+  constexpr int NW = NT / 64, U = 4, W = Chunk<T>::W, STEP = NT * W;
+  const unsigned group = group_of<NT>();
+  if (NT == 64 && group >= L.B * L.S) return;
+  const unsigned row = NT == 64 || LOGPROB ? group : group / (unsigned)pieces;
   const int64_t b = L.sequence_of(row), s0 = L.token_of(row);
-  if (L.target_of(b, s0) < 0) return;
+  const int tid = thread_of<NT>(), t = (int)L.target_of(b, s0);
+  if (t < 0) {
+    if (LOGPROB && tid == 0) {
+      logp[row] = 0.f;
+      rows[row] = RowState{0.f, 0.f, 0.f, 0.f};
+    }
+    return;
+  }
   const T* x = L.row<T>(b, s0);
-  const int V = (int)L.V, begin = (int)(blockIdx.x % (unsigned)pieces) * span, end = min(begin + span, whole<T>(V));
+  const int V = (int)L.V, begin = NT == 64 || LOGPROB ? 0 : (int)(group % (unsigned)pieces) * span;
+  const int end = NT == 64 || LOGPROB ? whole<T>(V) : min(begin + span, whole<T>(V));
+  const float zt = LOGPROB ? (float)x[t] : 0.f;
   float m = -INFINITY, s = 0.f;
-  for (int c0 = begin + threadIdx.x * W; c0 < end; c0 += STEP * U) {
+  for (int c0 = begin + tid * W; c0 < end; c0 += STEP * U) {
     Chunk<T> r[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -206,17 +244,16 @@ __global__ void __launch_bounds__(kLseThreads) lse_partial_kernel(Logits L, Scal
     s = s * c.of_exp(m - ms) + e;
     m = mn;
   }
-  if (begin + span >= V && threadIdx.x < V - whole<T>(V)) add_one((float)x[whole<T>(V) + threadIdx.x], c, &m, &s);
+  if (begin + span >= V && tid < V - whole<T>(V)) add_one((float)x[whole<T>(V) + tid], c, &m, &s);
   const RowSum all = block_join<NW>(m, s, c);
-  if (threadIdx.x == 0) part[blockIdx.x] = all;
-}
-
-// Log-probability of the token with logit zt from its row's (M, S), in fp64; a row of nothing but -inf, or with a NaN or
-// +inf, gives NaN.
-__device__ __forceinline__ double row_logprob(float zt, float M, double S, double inv_temp, float* l2s) {
-  const double l2 = log2(S);
-  *l2s = (float)l2;
-  return ((double)zt - (double)M) * inv_temp - l2 * 0.69314718055994530942;
+  if (tid != 0) return;
+  if (LOGPROB) {
+    RowState st{all.M, 0.f, 1.f, 0.f};
+    logp[row] = (float)row_logprob(zt, all.M, all.S, inv_temp, &st.l2s);
+    rows[row] = st;
+  } else {
+    part[group] = all;
+  }
 }
 
 // A group of `lanes` (a power of two, at least `pieces`) joins its row's pieces: (M, S) in every lane of the group
@@ -323,20 +360,19 @@ struct TokenInputs {
 };
 
 // One token: the loss term, and its slope by lp.  min(r A, clip(r) A) has slope r A except where the clipped term is the
-// smaller one: A > 0 above the upper bound, A < 0 below the lower one.
-__device__ __forceinline__ void policy_token(const PolicyArgs& a, const TokenInputs& in, double lp, double* loss,
-                                             double* slope, double* kl, bool* clipped) {
+// smaller one: A > 0 above the upper bound, A < 0 below the lower one.  r = exp(lp - old), q = exp(ref - lp): the KL term
+// q - 1 - d is exact to 2^-52 absolutely, far below what the rounding of ref_logp to fp32 does to it.
+__device__ __forceinline__ void policy_token(const PolicyArgs& a, const TokenInputs& in, double lp, double r, double q,
+                                             double* loss, double* slope, double* kl, bool* clipped) {
   const double A = (double)in.adv;
-  const double r = exp(lp - (double)in.old_logp);
   *clipped = (A > 0.0 && r > a.high) || (A < 0.0 && r < a.low);
   const double rc = *clipped ? (A > 0.0 ? a.high : a.low) : r;
   *loss = -rc * A;
   *slope = *clipped ? 0.0 : -r * A;
   *kl = 0.0;
   if (in.has_ref) {
-    const double d = (double)in.ref_logp - lp;
-    const double e = expm1(d);
-    *kl = e - d;
+    const double d = (double)in.ref_logp - lp, e = q - 1.0;
+    *kl = e < d ? 0.0 : e - d;  // (never below 0, rounded or not)
     if (a.kl_coef != 0.0) {
       *loss += a.kl_coef * *kl;
       *slope -= a.kl_coef * e;
@@ -362,7 +398,8 @@ __global__ void __launch_bounds__(256) policy_rows_kernel(Logits L, const RowSum
       lp = row_logprob((float)L.row<T>(b, s)[t], st.M, S, inv_temp, &st.l2s);
       double slope;
       bool clipped;
-      policy_token(a, TokenInputs(a, b, s), lp, &v[0], &slope, &v[1], &clipped);
+      const TokenInputs in(a, b, s);
+      policy_token(a, in, lp, exp(lp - (double)in.old_logp), exp((double)in.ref_logp - lp), &v[0], &slope, &v[1], &clipped);
       v[2] = clipped ? 1.0 : 0.0;
       v[3] = 1.0;
       st.coef = (float)slope;
@@ -454,7 +491,7 @@ __global__ void __launch_bounds__(256) pair_total_kernel(const double* __restric
 
 // ------------------------------------------------------------------ gradient of the logits
 constexpr int kGradThreads = 256, kGradChunks = 4;
-template <typename T> constexpr int kGradSpan = kGradThreads * kGradChunks * Chunk<T>::W;  // logits of one workgroup
+template <typename T, int NT = kGradThreads> constexpr int kGradSpan = NT * kGradChunks * Chunk<T>::W;  // logits of a unit
 
 // -k 2^((z - M) c - log2 s): dz without the k that the target's logit gets on top
 __device__ __forceinline__ float grad_of(float z, float M, float l2s, float k, const Scale& c) {
@@ -468,7 +505,7 @@ __device__ __forceinline__ void write_grad(Chunk<T> (&r)[CHUNKS], T* out, int be
   constexpr int W = Chunk<T>::W;
 #pragma unroll
   for (int u = 0; u < CHUNKS; ++u) {
-    const int cc = begin + (u * NT + (int)threadIdx.x) * W;
+    const int cc = begin + (u * NT + thread_of<NT>()) * W;
     if (cc < whole<T>(V)) {
 #pragma unroll
       for (int j = 0; j < W; ++j) r[u].set(j, grad_of(r[u].get(j), M, l2s, k, c));
@@ -482,7 +519,7 @@ __device__ __forceinline__ void write_grad(Chunk<T> (&r)[CHUNKS], T* out, int be
 template <typename T, int NT>
 __device__ __forceinline__ void write_target(T* out, int V, int t, float zt, float M, float l2s, float k, const Scale& c) {
   const int owner = t < whole<T>(V) ? t / Chunk<T>::W % NT : t - whole<T>(V);
-  if ((int)threadIdx.x == owner) {
+  if (thread_of<NT>() == owner) {
     const float d = zt - M;
     out[t] = (T)((1.f - exp2_(fmaf(d, c.hi, fmaf(d, c.lo, -l2s)))) * k);
   }
@@ -494,7 +531,7 @@ __device__ __forceinline__ void write_zeros(T* out, int begin, int V) {
   for (int j = 0; j < Chunk<T>::W; ++j) zero.set(j, 0.f);
 #pragma unroll
   for (int u = 0; u < CHUNKS; ++u) {
-    const int cc = begin + (u * NT + (int)threadIdx.x) * Chunk<T>::W;
+    const int cc = begin + (u * NT + thread_of<NT>()) * Chunk<T>::W;
     if (cc < whole<T>(V)) zero.store(out, cc);
   }
 }
@@ -503,22 +540,22 @@ __device__ __forceinline__ void write_zeros(T* out, int begin, int V) {
 // written in the forward for gout = 1, so nothing is left to do where that is what came.  Bound by the read and the write:
 // 6.4 TB/s at 8192 x 50304 bf16 (256 us), 6.2 at 1999 x 128256 fp32 (332 us).  Reading the rows from the last to the
 // first, for what the forward left in the Infinity Cache, changed nothing (425 us with the forward, 417 as it is).
-template <typename T>
+template <typename T, int NT>
 __global__ void __launch_bounds__(kGradThreads) logit_grad_kernel(Logits L, Scale c, const RowState* __restrict__ rows,
                                                                   const float* __restrict__ weight, TokenArray gout,
                                                                   float inv_temp, int spans, int64_t units,
                                                                   int unless_one, T* __restrict__ dz) {
   if (unless_one && *gout.p == 1.f) return;
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+  for (int64_t u = group_of<NT>(); u < units; u += gridDim.x * kRows<NT>) {
     const unsigned unit = (unsigned)u, row = unit / (unsigned)spans;  // (units are below 2^31)
     const int64_t b = L.sequence_of(row), s0 = L.token_of(row);
-    const int begin = (int)(unit % (unsigned)spans) * kGradSpan<T>, V = (int)L.V, t = (int)L.target_of(b, s0);
+    const int begin = (int)(unit % (unsigned)spans) * kGradSpan<T, NT>, V = (int)L.V, t = (int)L.target_of(b, s0);
     // the lane's logit behind the last whole chunk, where it has one and the span reaches there
-    const int last = whole<T>(V) + (int)threadIdx.x;
-    const bool tail = last < V && whole<T>(V) - begin < kGradSpan<T> && whole<T>(V) >= begin;
+    const int last = whole<T>(V) + thread_of<NT>();
+    const bool tail = last < V && whole<T>(V) - begin < kGradSpan<T, NT> && whole<T>(V) >= begin;
     T* out = dz + (int64_t)row * L.V;
     if (t < 0) {
-      write_zeros<T, kGradChunks, kGradThreads>(out, begin, V);
+      write_zeros<T, kGradChunks, NT>(out, begin, V);
       if (tail) out[last] = (T)0.f;
       continue;
     }
@@ -526,15 +563,15 @@ __global__ void __launch_bounds__(kGradThreads) logit_grad_kernel(Logits L, Scal
     Chunk<T> r[kGradChunks];
 #pragma unroll
     for (int u = 0; u < kGradChunks; ++u) {
-      const int cc = begin + (u * kGradThreads + (int)threadIdx.x) * Chunk<T>::W;
+      const int cc = begin + (u * NT + thread_of<NT>()) * Chunk<T>::W;
       if (cc < whole<T>(V)) r[u].load(x, cc);
     }
     const RowState st = rows[row];
     const float k = st.coef * (weight ? weight[b] : 1.f) * gout.at(b, s0) * inv_temp;
-    write_grad<T, kGradChunks, kGradThreads>(r, out, begin, V, st.M, st.l2s, k, c);
+    write_grad<T, kGradChunks, NT>(r, out, begin, V, st.M, st.l2s, k, c);
     if (tail) out[last] = (T)grad_of((float)x[last], st.M, st.l2s, k, c);
-    if (t >= begin && t - begin < kGradSpan<T>)
-      write_target<T, kGradThreads>(out, V, t, (float)x[t], st.M, st.l2s, k, c);
+    if (t >= begin && t - begin < kGradSpan<T, NT>)
+      write_target<T, NT>(out, V, t, (float)x[t], st.M, st.l2s, k, c);
   }
 }
 
@@ -565,8 +602,13 @@ __global__ void __launch_bounds__(1024) policy_weight_kernel(Logits L, int by_se
   } else {
     int n = 0;
     const unsigned N = (unsigned)(L.B * L.S);
+    if (L.tb == L.S * L.ts || L.B == 1) {  // one stride over all of them: no division for each
 #pragma unroll 8
-    for (unsigned i = threadIdx.x; i < N; i += 1024) n += L.target_of(L.sequence_of(i), L.token_of(i)) >= 0 ? 1 : 0;
+      for (unsigned i = threadIdx.x; i < N; i += 1024) n += L.target_of(0, i) >= 0 ? 1 : 0;
+    } else {
+#pragma unroll 8
+      for (unsigned i = threadIdx.x; i < N; i += 1024) n += L.target_of(L.sequence_of(i), L.token_of(i)) >= 0 ? 1 : 0;
+    }
     v[0] = (double)n;
   }
   block_sums64<1, 16>(v);
@@ -574,6 +616,13 @@ __global__ void __launch_bounds__(1024) policy_weight_kernel(Logits L, int by_se
     for (int64_t b = threadIdx.x; b < L.B; b += 1024) weight[b] = (float)(scale / (v[0] > 1.0 ? v[0] : 1.0));
   if (threadIdx.x == 0) *count = v[0];
 }
+
+// What a row adds to the loss (times the row's weight), to the mean KL (held in fp32, which the mean is returned in) and to
+// the count of clipped tokens
+struct PolicyTerms {
+  double loss;
+  float kl, clipped;
+};
 
 // Running (m, s) of a thread over its chunks of a row
 template <typename T, int NT, int N>
@@ -584,14 +633,14 @@ __device__ __forceinline__ void add_chunks(Chunk<T> (&r)[N], int V, const Scale&
     float mn = *m;
 #pragma unroll
     for (int u = g; u < (g + G < N ? g + G : N); ++u)
-      if ((u * NT + (int)threadIdx.x) * W < whole<T>(V))
+      if ((u * NT + thread_of<NT>()) * W < whole<T>(V))
 #pragma unroll
         for (int j = 0; j < W; ++j) mn = fmaxf(mn, r[u].get(j));
     const float ms = mn == -INFINITY ? 0.f : mn;
     float e = 0.f;
 #pragma unroll
     for (int u = g; u < (g + G < N ? g + G : N); ++u)
-      if ((u * NT + (int)threadIdx.x) * W < whole<T>(V)) e += exp_sum(r[u], ms, c);
+      if ((u * NT + thread_of<NT>()) * W < whole<T>(V)) e += exp_sum(r[u], ms, c);
     *s = *s * c.of_exp(*m - ms) + e;
     *m = mn;
     __builtin_amdgcn_sched_barrier(0);  // one group's fp32 values at a time: registers
@@ -601,24 +650,26 @@ __device__ __forceinline__ void add_chunks(Chunk<T> (&r)[N], int V, const Scale&
 }
 
 // One workgroup a row, the row in registers between its two uses (NT * CHUNKS chunks, at least the row's): one read and
-// one write of the logits' size.  terms[row]: {weighted loss, kl, clipped}.  It ran at 4.6-5.1 TB/s until less arithmetic
+// one write of the logits' size.  It ran at 4.6-5.1 TB/s until less arithmetic
 // and fewer registers a row brought 5.6-5.9 of the copy's 6.1; what is left is the time that a row's terms keep its
 // workgroup waiting.
 template <typename T, int NT, int CHUNKS, int WAVES>  // WAVES a SIMD that the registers leave room for
-__global__ void __launch_bounds__(NT, WAVES) policy_fused_kernel(Logits L, Scale c, double inv_temp, PolicyArgs a,
+__global__ void __launch_bounds__(NT * kRows<NT>, WAVES) policy_fused_kernel(Logits L, Scale c, double inv_temp, PolicyArgs a,
                                                                  const float* __restrict__ weight,
                                                                  float* __restrict__ logp, RowState* __restrict__ rows,
-                                                                 double4* __restrict__ terms, T* __restrict__ dz) {
-  const int64_t row = blockIdx.x, b = L.sequence_of(blockIdx.x), s0 = L.token_of(blockIdx.x);
-  const int V = (int)L.V, t = (int)L.target_of(b, s0), last = whole<T>(V) + (int)threadIdx.x;
+                                                                 PolicyTerms* __restrict__ terms, T* __restrict__ dz) {
+  const unsigned group = group_of<NT>();
+  if (NT == 64 && group >= L.B * L.S) return;
+  const int64_t row = group, b = L.sequence_of(group), s0 = L.token_of(group);
+  const int tid = thread_of<NT>(), V = (int)L.V, t = (int)L.target_of(b, s0), last = whole<T>(V) + tid;
   T* out = dz + row * L.V;
   if (t < 0) {
     write_zeros<T, CHUNKS, NT>(out, 0, V);
     if (last < V) out[last] = (T)0.f;
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
       logp[row] = 0.f;
       rows[row] = RowState{0.f, 0.f, 0.f, 0.f};
-      terms[row] = make_double4(0.0, 0.0, 0.0, 0.0);
+      terms[row] = {0.0, 0.f, 0.f};
     }
     return;
   }
@@ -630,7 +681,7 @@ __global__ void __launch_bounds__(NT, WAVES) policy_fused_kernel(Logits L, Scale
   Chunk<T> r[CHUNKS];
 #pragma unroll
   for (int u = 0; u < CHUNKS; ++u) {  // every load in flight before any use
-    const int cc = (u * NT + (int)threadIdx.x) * Chunk<T>::W;
+    const int cc = (u * NT + tid) * Chunk<T>::W;
     if (cc < whole<T>(V)) r[u].load(x, cc);
   }
   in.to_scalar();
@@ -639,39 +690,51 @@ __global__ void __launch_bounds__(NT, WAVES) policy_fused_kernel(Logits L, Scale
   float m = -INFINITY, s = 0.f;
   add_chunks<T, NT>(r, V, c, &m, &s);
   add_one(tail, c, &m, &s);
-  __shared__ float pass[3];
   const RowSum all = block_join<NT / 64>(m, s, c);
-  if (threadIdx.x == 0) {
-    RowState st{all.M, 0.f, 0.f, 0.f};
-    const double lp = row_logprob(zt, all.M, all.S, inv_temp, &st.l2s);
+  const float M = scalar(all.M);
+  float l2s = 0.f, k = 0.f;
+  if (tid < 64) {  // the first wave: the same in all lanes but for the exponential, r in the even ones, q in the odd ones
+    const double lp = row_logprob(zt, M, all.S, inv_temp, &l2s);
+    const double d = tid & 1 ? (double)in.ref_logp - lp : lp - (double)in.old_logp, e = exp(d);
     double loss, slope, kl;
     bool clipped;
-    policy_token(a, in, lp, &loss, &slope, &kl, &clipped);
-    st.coef = (float)slope;
-    pass[0] = st.M;
-    pass[1] = st.l2s;
-    pass[2] = st.coef * w * (float)inv_temp;
-    logp[row] = (float)lp;
-    rows[row] = st;
-    terms[row] = make_double4(loss * (double)w, kl, clipped ? 1.0 : 0.0, 0.0);
+    policy_token(a, in, lp, __shfl(e, 0, kWave), __shfl(e, 1, kWave), &loss, &slope, &kl, &clipped);
+    const RowState st{M, l2s, (float)slope, 0.f};
+    k = st.coef * w * (float)inv_temp;
+    if (tid == 0) {
+      logp[row] = (float)lp;
+      rows[row] = st;
+      terms[row] = {loss * (double)w, (float)kl, clipped ? 1.f : 0.f};
+    }
   }
-  __syncthreads();
-  const float M = pass[0], l2s = pass[1], k = pass[2];
+  if constexpr (NT == 64) {  // the wave's first lane has them
+    l2s = scalar(l2s);
+    k = scalar(k);
+  } else {
+    __shared__ float pass[2];
+    if (tid == 0) {
+      pass[0] = l2s;
+      pass[1] = k;
+    }
+    __syncthreads();
+    l2s = scalar(pass[0]);
+    k = scalar(pass[1]);
+  }
   write_grad<T, CHUNKS, NT>(r, out, 0, V, M, l2s, k, c);
   if (last < V) out[last] = (T)grad_of(tail, M, l2s, k, c);
   write_target<T, NT>(out, V, t, zt, M, l2s, k, c);
 }
 
-__global__ void __launch_bounds__(1024) policy_sum_kernel(const double4* __restrict__ terms, int64_t N,
+__global__ void __launch_bounds__(1024) policy_sum_kernel(const PolicyTerms* __restrict__ terms, int64_t N,
                                                           const double* __restrict__ count, float* __restrict__ loss,
                                                           float* __restrict__ stats) {
   double v[3] = {0.0, 0.0, 0.0};
 #pragma unroll 8
   for (unsigned i = threadIdx.x; i < (unsigned)N; i += 1024) {
-    const double4 x = terms[i];
-    v[0] += x.x;
-    v[1] += x.y;
-    v[2] += x.z;
+    const PolicyTerms x = terms[i];
+    v[0] += x.loss;
+    v[1] += (double)x.kl;
+    v[2] += (double)x.clipped;
   }
   block_sums64<3, 16>(v);
   if (threadIdx.x == 0) {
@@ -704,10 +767,25 @@ static LseShape lse_shape(int64_t N, int64_t V) {
 }
 static int64_t segments(int64_t S, const LseShape& sh) { return (S * sh.lanes + 255) / 256; }
 
+// A wave a row, in the sums and in the gradient: short rows, enough of them.  Sums of rows in us, workgroup / wave a row:
+// bf16, 24000 rows of 1003 32.0 / 16.1, of 2000 34.8 / 20.6, of 4000 40.8 / 31.7; 2000 rows of 1003 4.8 / 4.0, of 4000
+// 6.1 / 6.0, 500 rows of 1003 3.4 / 3.6, of 4000 3.6 / 4.8; fp32, 24000 rows of 2000 34.2 / 29.6, of 4000 61.0 / 57.7, but
+// 4000 of them 9.7 / 11.5.  Gradient, 24000 rows: bf16 of 1003 40.0 / 21.9, of 2000 43.4 / 33.8, fp32 of 1003 42.9 / 35.1.
+constexpr int64_t kWaveRows = 2000;
+template <typename T>
+static bool wave_sums(const Logits& L) { return L.B * L.S >= kWaveRows && L.V <= 2 * kGradSpan<T, 64>; }
+template <typename T>
+static bool wave_grads(const Logits& L) { return L.B * L.S >= kWaveRows && L.V <= kGradSpan<T, 64>; }
+
 template <typename T>
 static hipError_t lse_partial(const Logits& L, const Scale& c, const LseShape& sh, RowSum* part, hipStream_t st) {
-  hipLaunchKernelGGL(lse_partial_kernel<T>, dim3((unsigned)(L.B * L.S * sh.pieces)), dim3(kLseThreads), 0, st, L, c,
-                     sh.pieces, sh.span, part);
+  const int64_t N = L.B * L.S;
+  if (wave_sums<T>(L))
+    hipLaunchKernelGGL((lse_partial_kernel<T, 64, false>), dim3((unsigned)((N + 3) / 4)), dim3(kLseThreads), 0, st, L, c,
+                       sh.pieces, sh.span, part, 0.0, nullptr, nullptr);
+  else
+    hipLaunchKernelGGL((lse_partial_kernel<T, kLseThreads, false>), dim3((unsigned)(N * sh.pieces)), dim3(kLseThreads), 0,
+                       st, L, c, sh.pieces, sh.span, part, 0.0, nullptr, nullptr);
   return hipGetLastError();
 }
 
@@ -754,9 +832,17 @@ hipError_t dta_pref_logprobs(const PrefLogits& l, int type, double temperature, 
   const LseShape sh = lse_shape(N, L.V);
   const Scale c = scale_of(temperature);
   DTA_BY_TYPE(type, {
-    DTA_HIP_CHECK(lse_partial<T>(L, c, sh, (RowSum*)part, st));
-    hipLaunchKernelGGL(logprob_rows_kernel<T>, dim3((unsigned)((N * sh.lanes + 255) / 256)), dim3(256), 0, st, L,
-                       (RowSum*)part, sh.pieces, sh.lanes, c, 1.0 / temperature, logp, (RowState*)rows);
+    if (wave_sums<T>(L)) {
+      hipLaunchKernelGGL((lse_partial_kernel<T, 64, true>), dim3((unsigned)((N + 3) / 4)), dim3(kLseThreads), 0, st, L, c,
+                         1, sh.span, nullptr, 1.0 / temperature, logp, (RowState*)rows);
+    } else if (sh.pieces == 1) {
+      hipLaunchKernelGGL((lse_partial_kernel<T, kLseThreads, true>), dim3((unsigned)N), dim3(kLseThreads), 0, st, L, c, 1,
+                         sh.span, nullptr, 1.0 / temperature, logp, (RowState*)rows);
+    } else {
+      DTA_HIP_CHECK(lse_partial<T>(L, c, sh, (RowSum*)part, st));
+      hipLaunchKernelGGL(logprob_rows_kernel<T>, dim3((unsigned)((N * sh.lanes + 255) / 256)), dim3(256), 0, st, L,
+                         (RowSum*)part, sh.pieces, sh.lanes, c, 1.0 / temperature, logp, (RowState*)rows);
+    }
   })
   return hipGetLastError();
 }
@@ -796,27 +882,30 @@ int dta_pref_policy_fused(int type, int64_t N, int64_t V) {
 
 template <typename T, int NT, int CHUNKS, int WAVES>
 static void policy_fused(const Logits& L, double temperature, const PrefPolicy& p, const float* weight, float* logp,
-                         void* rows, double* terms, void* dz, hipStream_t st) {
-  hipLaunchKernelGGL((policy_fused_kernel<T, NT, CHUNKS, WAVES>), dim3((unsigned)(L.B * L.S)), dim3(NT), 0, st, L,
+                         void* rows, void* terms, void* dz, hipStream_t st) {
+  hipLaunchKernelGGL((policy_fused_kernel<T, NT, CHUNKS, WAVES>), dim3((unsigned)((L.B * L.S + kRows<NT> - 1) / kRows<NT>)),
+                     dim3(NT * kRows<NT>), 0, st, L,
                      scale_of(temperature), 1.0 / temperature, policy_args(p), weight, logp, (RowState*)rows,
-                     (double4*)terms, (T*)dz);
+                     (PolicyTerms*)terms, (T*)dz);
 }
 
-hipError_t dta_pref_policy_grad(const PrefLogits& l, int type, double temperature, const PrefPolicy& p, double* terms,
+hipError_t dta_pref_policy_grad(const PrefLogits& l, int type, double temperature, const PrefPolicy& p, void* terms,
                                 float* loss, float* stats, float* logp, void* rows, float* weight, void* dz,
                                 hipStream_t st) {
   const Logits L = logits_of(l);
   const int64_t N = L.B * L.S;
   if (!dta_pref_policy_fused(type, N, L.V)) return hipErrorInvalidValue;
-  double* count = terms + 4 * N;
+  double* count = (double*)((PolicyTerms*)terms + N);
   hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, L, p.by_sequence, p.scale, weight, count);
   DTA_HIP_CHECK(hipGetLastError());
   // Threads and 16-byte chunks a thread by the row's size: as many rows on a CU as its registers hold (V = 50304 in bf16:
-  // 1024 x 7 at 8 waves a SIMD 279 us, 512 x 13 287, 256 x 25 306, 1024 x 7 at 4 waves 367, for 8192 rows)
+  // 1024 x 7 at 8 waves a SIMD 279 us, 512 x 13 287, 256 x 25 306, 1024 x 7 at 4 waves 367, for 8192 rows).  A wave a row
+  // for the shortest: 24000 rows of 2000 in bf16 64 x 4 38.5 us, 256 x 2 51.2; of 4000 64 x 8 69.8, 256 x 2 67.8.
 #define DTA_FUSED(T, NT, CHUNKS, WAVES) \
   policy_fused<T, NT, CHUNKS, WAVES>(L, temperature, p, weight, logp, rows, terms, dz, st)
 #define DTA_FUSED_ANY(T, W)                                   \
   if (L.V <= W * 64 * 2) DTA_FUSED(T, 64, 2, 8);              \
+  else if (L.V <= W * 64 * 4) DTA_FUSED(T, 64, 4, 8);         \
   else if (L.V <= W * 256 * 2) DTA_FUSED(T, 256, 2, 8);       \
   else if (L.V <= W * 256 * 4) DTA_FUSED(T, 256, 4, 8);       \
   else if (L.V <= W * 512 * 4) DTA_FUSED(T, 512, 4, 8);       \
@@ -836,7 +925,7 @@ hipError_t dta_pref_policy_grad(const PrefLogits& l, int type, double temperatur
 #undef DTA_FUSED_ANY
 #undef DTA_FUSED
   DTA_HIP_CHECK(hipGetLastError());
-  hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(1024), 0, st, (double4*)terms, N, count, loss, stats);
+  hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(1024), 0, st, (PolicyTerms*)terms, N, count, loss, stats);
   return hipGetLastError();
 }
 
@@ -867,13 +956,19 @@ hipError_t dta_pref_grad(const PrefLogits& l, int type, double temperature, cons
   const int64_t N = L.B * L.S;
   if (N == 0) return hipSuccess;
   DTA_BY_TYPE(type, {
-    const int spans = (int)((L.V + kGradSpan<T> - 1) / kGradSpan<T>);
-    const int64_t units = N * spans;
+    const float inv = (float)(1.0 / temperature);
     // (a launch that is expected to end at once is a small one, whose workgroups walk over the rows if they have to)
-    const int64_t grid = min(units, unless_one ? (int64_t)2048 : kMostGroups);
-    hipLaunchKernelGGL(logit_grad_kernel<T>, dim3((unsigned)grid), dim3(kGradThreads), 0, st, L, scale_of(temperature),
-                       (const RowState*)rows, weight, array_of(gout), (float)(1.0 / temperature), spans, units,
-                       unless_one, (T*)dz);
+    const int64_t most = unless_one ? 2048 : kMostGroups;
+    if (wave_grads<T>(L)) {
+      hipLaunchKernelGGL((logit_grad_kernel<T, 64>), dim3((unsigned)min((N + 3) / 4, most)), dim3(kGradThreads), 0, st, L,
+                         scale_of(temperature), (const RowState*)rows, weight, array_of(gout), inv, 1, N, unless_one,
+                         (T*)dz);
+    } else {
+      const int spans = (int)((L.V + kGradSpan<T> - 1) / kGradSpan<T>);
+      hipLaunchKernelGGL((logit_grad_kernel<T, kGradThreads>), dim3((unsigned)min(N * spans, most)), dim3(kGradThreads), 0,
+                         st, L, scale_of(temperature), (const RowState*)rows, weight, array_of(gout), inv, spans,
+                         N * spans, unless_one, (T*)dz);
+    }
   })
   return hipGetLastError();
 }

@@ -421,7 +421,7 @@ def test_many_rows_of_a_tiny_vocabulary():
         x = z.detach()[:n].requires_grad_()
         old, adv = torch.full((n,), want, device=DEV), torch.ones(n, device=DEV)
         out = preference.policy_loss(x, target[:n], old, adv)
-        assert abs(float(out.loss) + 1.0) < 1e-6 and float(out.clip_fraction) == 0.0
+        assert abs(float(out.loss.detach()) + 1.0) < 1e-6 and float(out.clip_fraction) == 0.0
         out.loss.backward()
         # k = -1 / n times [-(1 - p), 1 - p], rounded to bf16
         slope = (1 - math.exp(want)) / n
@@ -506,3 +506,50 @@ def test_extreme_logits_in_one_pass(V):
     lp, g = grads(z, 600, 600.0)
     assert torch.isnan(lp[0, 3:6]).all() and torch.isnan(g[0, 3:6]).all()
     assert torch.isfinite(lp[0, 6:]).all() and torch.isfinite(g[0, 6:]).all() and torch.isfinite(g[0, :3]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [1, 7, 8, 9, 63, 512, 513, 1024, 1025, 2047, 2048, 2049, 4096, 4097])
+def test_short_rows(V, dtype):
+    """From 2000 rows on a short row is one wave's: the operators at the sizes around its limits, rows not in fours."""
+    test_token_logprobs(3, 667, V, dtype, 0.7)
+    test_policy_loss(3, 667, V, dtype, 0.1, 0.28, "sequence", 0.25)
+    test_preference_loss(2, 1001, V, dtype, 0.1, True, False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [900, 2000, 4000])
+def test_extreme_logits_in_short_rows(V, dtype):
+    """Rows of -inf, of the type's lowest value, of NaN and inf, of strided logits: a wave a row as a workgroup a row."""
+    N = 2003
+    wide = torch.randn(N, V + 5, generator=torch.Generator().manual_seed(V)).to(dtype).to(DEV)
+    z = wide[:, 3:3 + V]
+    target = torch.randint(V, (N,), generator=torch.Generator().manual_seed(1)).to(DEV)
+    target[7], target[8], target[2002] = -100, V, -1
+    low = torch.finfo(dtype).min
+    z[0, : V - 1], z[1], z[2, : V // 2], z[3] = float("-inf"), low, low, float("-inf")
+    z[4, 5], z[5, V - 1], z[7], z[2002] = float("nan"), float("inf"), float("nan"), float("nan")
+    target[0] = V - 1
+    got = []
+    for n in (N, 40):
+        x = z[:n].detach().requires_grad_()
+        lp = preference.token_logprobs(x, target[:n], temperature=0.7)
+        got.append((lp.detach(), torch.autograd.grad(lp.sum(), x)[0]))
+    (lp, g), (lp_few, g_few) = got
+    assert float(lp[0]) == 0.0 and abs(float(lp[1]) + math.log(V)) < 1e-5
+    bad = torch.isin(torch.arange(40, device=DEV), torch.tensor([3, 4, 5], device=DEV))
+    assert torch.isnan(lp[3:6]).all() and torch.isnan(g[3:6]).all()
+    for row in (7, 8, 2002):
+        assert float(lp[row]) == 0.0 and not g[row].any()
+    assert torch.isfinite(lp[6:]).all() and torch.isfinite(g[6:]).all()
+    live = ~bad & (target[:40] >= 0) & (target[:40] < V)
+    # both forms are within stat_error of the same value; rows 0 and 1 are exact or uniform; row 2's lowest entries add
+    # exactly 0 (2^-inf), the others make an ordinary row of it (a target among the lowest: lp is -inf or near it in both)
+    e = torch.zeros(40, 1, device=DEV, dtype=torch.float64)
+    e[6:] = oracle.stat_error(torch.nan_to_num(z[6:40].double()), 0.7)
+    e[:2] = 2.0 ** -20
+    e[2] = oracle.stat_error(z[2:3, V // 2:].double(), 0.7)
+    near = (lp[:40] - lp_few).abs() <= 2 * e[:, 0] + lp_few.abs() * 2.0 ** -23
+    assert (near | (lp[:40] == lp_few))[live].all()
+    tol = g_few.double().abs() * (2 * oracle.half_step(dtype) * 1.01 + 2 * e) + oracle.smallest(dtype) * 2
+    assert ((g[:40].double() - g_few.double()).abs() <= tol + 2 * e / 0.7)[live].all()
