@@ -5,9 +5,9 @@
 //   lp = (z_y - M) / temperature - ln s                              log-probability of the token y
 //   dz_j = k ([j = y] - 2^((z_j - M) c - log2 s)),  k = dloss/dlp / temperature
 //
-// Three steps: every row's (M, s) (lse_partial_kernel, one pass over the logits, a row cut into pieces where there
-// are few); the rows' terms and the loss (one thread a row, then one workgroup); dz (logit_grad_kernel, a second
-// read of the logits and a write).  Both passes over the logits wait for memory.  The policy loss of many rows takes
+// Three steps: every row's (M, s) (lse_partial_kernel, one pass over the logits, a long row cut into pieces where there
+// are few); the rows' terms and the loss (one thread a row, in the same kernel or after it, then one workgroup); dz
+// (logit_grad_kernel, a second read of the logits and a write).  Both passes over the logits wait for memory.  The policy loss of many rows takes
 // one pass instead (policy_fused_kernel): all that a row's gradient needs is known once its own sum is.
 //
 // The row's maximum is subtracted before the multiplication by c, not folded into one fma: rows of the type's lowest
@@ -138,7 +138,7 @@ __device__ __forceinline__ unsigned group_of() {  // among all groups of NT thre
   return NT == 64 ? blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
 }
 
-constexpr int kLseThreads = 256;
+constexpr int kLseThreads = 256, kLongThreads = 1024;
 
 template <int CTRL, int ROWMASK>
 __device__ __forceinline__ double dpp_mov64(double v) {  // lanes outside ROWMASK get 0
@@ -198,64 +198,6 @@ __device__ __forceinline__ double row_logprob(float zt, float M, double S, doubl
   return ((double)zt - (double)M) * inv_temp - l2 * 0.69314718055994530942;
 }
 
-// Group row * pieces + i: piece i of the row, [i * span, (i + 1) * span).  U chunks a thread are requested before
-// any is used and share one rescaling of the running sum.  Bound by the read: 6.7 TB/s at 8192 x 50304 bf16 (123 us), 6.7
-// at 1999 x 128256 fp32 (153 us).
-// LOGPROB (rows of one piece): the row's log-probability and state as well, which spares logprob_rows_kernel.
-template <typename T, int NT, bool LOGPROB>
-__global__ void __launch_bounds__(kLseThreads) lse_partial_kernel(Logits L, Scale c, int pieces, int span,
-                                                                  RowSum* __restrict__ part, double inv_temp,
-                                                                  float* __restrict__ logp,
-                                                                  RowState* __restrict__ rows) {
-  constexpr int NW = NT / 64, U = 4, W = Chunk<T>::W, STEP = NT * W;
-  const unsigned group = group_of<NT>();
-  if (NT == 64 && group >= L.B * L.S) return;
-  const unsigned row = NT == 64 || LOGPROB ? group : group / (unsigned)pieces;
-  const int64_t b = L.sequence_of(row), s0 = L.token_of(row);
-  const int tid = thread_of<NT>(), t = (int)L.target_of(b, s0);
-  if (t < 0) {
-    if (LOGPROB && tid == 0) {
-      logp[row] = 0.f;
-      rows[row] = RowState{0.f, 0.f, 0.f, 0.f};
-    }
-    return;
-  }
-  const T* x = L.row<T>(b, s0);
-  const int V = (int)L.V, begin = NT == 64 || LOGPROB ? 0 : (int)(group % (unsigned)pieces) * span;
-  const int end = NT == 64 || LOGPROB ? whole<T>(V) : min(begin + span, whole<T>(V));
-  const float zt = LOGPROB ? (float)x[t] : 0.f;
-  float m = -INFINITY, s = 0.f;
-  for (int c0 = begin + tid * W; c0 < end; c0 += STEP * U) {
-    Chunk<T> r[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c0 + u * STEP < end) r[u].load(x, c0 + u * STEP);
-    float mn = m;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c0 + u * STEP < end)
-#pragma unroll
-        for (int j = 0; j < W; ++j) mn = fmaxf(mn, r[u].get(j));
-    const float ms = mn == -INFINITY ? 0.f : mn;  // nothing but -inf so far: the sum stays 0, not NaN
-    float e = 0.f;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c0 + u * STEP < end) e += exp_sum(r[u], ms, c);
-    s = s * c.of_exp(m - ms) + e;
-    m = mn;
-  }
-  if (begin + span >= V && tid < V - whole<T>(V)) add_one((float)x[whole<T>(V) + tid], c, &m, &s);
-  const RowSum all = block_join<NW>(m, s, c);
-  if (tid != 0) return;
-  if (LOGPROB) {
-    RowState st{all.M, 0.f, 1.f, 0.f};
-    logp[row] = (float)row_logprob(zt, all.M, all.S, inv_temp, &st.l2s);
-    rows[row] = st;
-  } else {
-    part[group] = all;
-  }
-}
-
 // A group of `lanes` (a power of two, at least `pieces`) joins its row's pieces: (M, S) in every lane of the group
 __device__ __forceinline__ void join_pieces(const RowSum* __restrict__ part, int pieces, int lanes, int64_t row,
                                             bool live, const Scale& c, float* M, double* S) {
@@ -293,24 +235,50 @@ __device__ __forceinline__ void block_sums64(double (&v)[K]) {
   __syncthreads();
 }
 
-// f(b, sums of sequence b's segments) for every sequence, by one 256-thread workgroup: a thread a sequence where they have
-// few segments, a wave a sequence (f in its first lane) where they have many
+// f(b, sums of sequence b's segments) for every sequence, by one workgroup of kTotalThreads: a thread a sequence where they
+// have few segments, else a wave or several a sequence
+constexpr int kTotalThreads = 1024;
 template <int K, typename F>
 __device__ __forceinline__ void for_each_sequence(const double* __restrict__ seg, int64_t B, int segs, F f) {
-  const bool waves = segs > 16;
-  const int lane = threadIdx.x & 63;
-  for (int64_t b = waves ? threadIdx.x >> 6 : threadIdx.x; b < B; b += waves ? 4 : 256) {
-    double q[K];
+  constexpr int NW = kTotalThreads / 64;
+  double q[K];
+  if (segs <= 16) {
+    for (int64_t b = threadIdx.x; b < B; b += kTotalThreads) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) q[k] = 0.0;
+      for (int i = 0; i < segs; ++i)
+#pragma unroll
+        for (int k = 0; k < K; ++k) q[k] += seg[(b * segs + i) * K + k];
+      f(b, q);
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, each = B > 0 && B < NW ? NW / (int)B : 1;
+  __shared__ double part[NW][K];
+  for (int64_t b = wave / each; b < B; b += NW / each) {  // (each > 1: at most once)
 #pragma unroll
     for (int k = 0; k < K; ++k) q[k] = 0.0;
-    for (int i = waves ? lane : 0; i < segs; i += waves ? 64 : 1)
+#pragma unroll 8
+    for (int i = wave % each * 64 + lane; i < segs; i += each * 64)
 #pragma unroll
       for (int k = 0; k < K; ++k) q[k] += seg[(b * segs + i) * K + k];
-    if (waves) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) q[k] = wave_sum64(q[k]);
+    for (int k = 0; k < K; ++k) q[k] = wave_sum64(q[k]);
+    if (lane == 0) {
+      if (each == 1) f(b, q);
+#pragma unroll
+      for (int k = 0; k < K; ++k) part[wave][k] = q[k];
     }
-    if (!waves || lane == 0) f(b, q);
+  }
+  if (each == 1) return;
+  __syncthreads();
+  if (threadIdx.x < B) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) q[k] = 0.0;
+    for (int w = 0; w < each; ++w)
+#pragma unroll
+      for (int k = 0; k < K; ++k) q[k] += part[threadIdx.x * each + w][k];
+    f(threadIdx.x, q);
   }
 }
 
@@ -349,6 +317,7 @@ __device__ __forceinline__ float scalar(float x) {
 struct TokenInputs {
   float old_logp, ref_logp, adv;
   bool has_ref;
+  TokenInputs() = default;
   __device__ __forceinline__ void to_scalar() {
     old_logp = scalar(old_logp);
     ref_logp = scalar(ref_logp);
@@ -380,6 +349,80 @@ __device__ __forceinline__ void policy_token(const PolicyArgs& a, const TokenInp
   }
 }
 
+// Group row * pieces + i: piece i of the row, [i * span, (i + 1) * span).  U chunks a thread are requested before
+// any is used and share one rescaling of the running sum.  Bound by the read: 6.7 TB/s at 8192 x 50304 bf16 (123 us), 6.9
+// at 1999 x 128256 fp32 (148 us).
+// What follows for rows of one piece is worked out here as well, which spares a launch: their log-probabilities, terms of
+// the policy loss (seg: a double4 a row, as policy_rows_kernel's), or terms of the pairs (a double2 a row).
+enum Then { kPieces, kLogprobs, kPolicy, kPairs };
+template <typename T, int NT, Then THEN>
+__global__ void __launch_bounds__(NT * kRows<NT>) lse_partial_kernel(Logits L, Scale c, int pieces, int span,
+                                                                  RowSum* __restrict__ part, double inv_temp,
+                                                                  PolicyArgs a, float* __restrict__ logp,
+                                                                  RowState* __restrict__ rows,
+                                                                  void* __restrict__ seg) {
+  constexpr bool WHOLE = NT == 64 || THEN != kPieces;
+  constexpr int NW = NT / 64, U = 4, W = Chunk<T>::W, STEP = NT * W;
+  const unsigned group = group_of<NT>();
+  if (NT == 64 && group >= L.B * L.S) return;
+  const unsigned row = WHOLE ? group : group / (unsigned)pieces;
+  const int64_t b = L.sequence_of(row), s0 = L.token_of(row);
+  const int tid = thread_of<NT>(), t = (int)L.target_of(b, s0);
+  if (t < 0) {
+    if (THEN == kPieces || tid != 0) return;
+    if (THEN == kLogprobs || THEN == kPolicy) logp[row] = 0.f;
+    rows[row] = RowState{0.f, 0.f, 0.f, 0.f};
+    if (THEN == kPolicy) static_cast<double4*>(seg)[row] = make_double4(0.0, 0.0, 0.0, 0.0);
+    if (THEN == kPairs) static_cast<double2*>(seg)[row] = make_double2(0.0, 0.0);
+    return;
+  }
+  const T* x = L.row<T>(b, s0);
+  const int V = (int)L.V, begin = WHOLE ? 0 : (int)(group % (unsigned)pieces) * span;
+  const int end = WHOLE ? whole<T>(V) : min(begin + span, whole<T>(V));
+  const float zt = THEN != kPieces ? (float)x[t] : 0.f;
+  TokenInputs in{};
+  if (THEN == kPolicy) in = TokenInputs(a, b, s0);
+  float m = -INFINITY, s = 0.f;
+  for (int c0 = begin + tid * W; c0 < end; c0 += STEP * U) {
+    Chunk<T> r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * STEP < end) r[u].load(x, c0 + u * STEP);
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * STEP < end)
+#pragma unroll
+        for (int j = 0; j < W; ++j) mn = fmaxf(mn, r[u].get(j));
+    const float ms = mn == -INFINITY ? 0.f : mn;  // nothing but -inf so far: the sum stays 0, not NaN
+    float e = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * STEP < end) e += exp_sum(r[u], ms, c);
+    s = s * c.of_exp(m - ms) + e;
+    m = mn;
+  }
+  if (begin + span >= V && tid < V - whole<T>(V)) add_one((float)x[whole<T>(V) + tid], c, &m, &s);
+  const RowSum all = block_join<NW>(m, s, c);
+  if (tid != 0) return;
+  if (THEN == kPieces) {
+    part[group] = all;
+    return;
+  }
+  RowState st{all.M, 0.f, 1.f, 0.f};
+  const double lp = row_logprob(zt, all.M, all.S, inv_temp, &st.l2s);
+  if (THEN == kPolicy) {
+    double loss, slope, kl;
+    bool clipped;
+    policy_token(a, in, lp, exp(lp - (double)in.old_logp), in.has_ref ? exp((double)in.ref_logp - lp) : 1.0, &loss, &slope, &kl, &clipped);
+    st.coef = (float)slope;
+    static_cast<double4*>(seg)[row] = make_double4(loss, kl, clipped ? 1.0 : 0.0, 1.0);
+  }
+  if (THEN == kPairs) static_cast<double2*>(seg)[row] = make_double2(lp, 1.0);
+  if (THEN == kLogprobs || THEN == kPolicy) logp[row] = (float)lp;
+  rows[row] = st;
+}
+
 // Workgroup b * segs + i: 256 / lanes tokens of sequence b.  seg: [B * segs] sums {loss, kl, clipped, tokens}.
 template <typename T>
 __global__ void __launch_bounds__(256) policy_rows_kernel(Logits L, const RowSum* __restrict__ part, int pieces,
@@ -399,7 +442,7 @@ __global__ void __launch_bounds__(256) policy_rows_kernel(Logits L, const RowSum
       double slope;
       bool clipped;
       const TokenInputs in(a, b, s);
-      policy_token(a, in, lp, exp(lp - (double)in.old_logp), exp((double)in.ref_logp - lp), &v[0], &slope, &v[1], &clipped);
+      policy_token(a, in, lp, exp(lp - (double)in.old_logp), in.has_ref ? exp((double)in.ref_logp - lp) : 1.0, &v[0], &slope, &v[1], &clipped);
       v[2] = clipped ? 1.0 : 0.0;
       v[3] = 1.0;
       st.coef = (float)slope;
@@ -412,7 +455,7 @@ __global__ void __launch_bounds__(256) policy_rows_kernel(Logits L, const RowSum
 }
 
 // stats: {kl, clip fraction}; weight[b]: what a token of sequence b counts in the loss
-__global__ void __launch_bounds__(256) policy_total_kernel(const double* __restrict__ seg, int64_t B, int segs,
+__global__ void __launch_bounds__(kTotalThreads) policy_total_kernel(const double* __restrict__ seg, int64_t B, int segs,
                                                            int by_sequence, double scale, float* __restrict__ loss,
                                                            float* __restrict__ stats, float* __restrict__ weight) {
   double v[4] = {0.0, 0.0, 0.0, 0.0};
@@ -424,10 +467,10 @@ __global__ void __launch_bounds__(256) policy_total_kernel(const double* __restr
     }
     for (int k = 0; k < 4; ++k) v[k] += q[k];
   });
-  block_sums64(v);
+  block_sums64<4, kTotalThreads / 64>(v);
   const double w = 1.0 / (v[3] > 1.0 ? v[3] : 1.0);
   if (!by_sequence)
-    for (int64_t b = threadIdx.x; b < B; b += 256) weight[b] = (float)(w * scale);
+    for (int64_t b = threadIdx.x; b < B; b += kTotalThreads) weight[b] = (float)(w * scale);
   if (threadIdx.x == 0) {
     *loss = (float)(v[0] * (by_sequence ? scale : w * scale));
     stats[0] = (float)(v[1] * w);
@@ -461,7 +504,7 @@ __global__ void __launch_bounds__(256) pair_rows_kernel(Logits L, const RowSum* 
 }
 
 // Pair p: sequences p (chosen) and p + P (rejected).  softplus(x) = max(x, 0) + log1p(exp(-|x|)).  total: [2 P] scratch.
-__global__ void __launch_bounds__(256) pair_total_kernel(const double* __restrict__ seg, int64_t P, int segs,
+__global__ void __launch_bounds__(kTotalThreads) pair_total_kernel(const double* __restrict__ seg, int64_t P, int segs,
                                                          const float* __restrict__ ref, int64_t ref_stride,
                                                          double beta, double smoothing, int average, double scale,
                                                          double2* __restrict__ total, float* __restrict__ loss,
@@ -474,7 +517,7 @@ __global__ void __launch_bounds__(256) pair_total_kernel(const double* __restric
   });
   __syncthreads();
   double v[1] = {0.0};
-  for (int64_t p = threadIdx.x; p < P; p += 256) {
+  for (int64_t p = threadIdx.x; p < P; p += kTotalThreads) {
     const double2 yes = total[p], no = total[p + P];
     const double r = ref ? (double)ref[p * ref_stride] - (double)ref[(p + P) * ref_stride] : 0.0;
     const double h = beta * (yes.x - no.x - r);
@@ -485,7 +528,7 @@ __global__ void __launch_bounds__(256) pair_total_kernel(const double* __restric
     weight[p] = (float)(slope * yes.y);
     weight[p + P] = (float)(-slope * no.y);
   }
-  block_sums64(v);
+  block_sums64<1, kTotalThreads / 64>(v);
   if (threadIdx.x == 0) *loss = (float)(scale * v[0] / (double)P);
 }
 
@@ -777,15 +820,46 @@ static bool wave_sums(const Logits& L) { return L.B * L.S >= kWaveRows && L.V <=
 template <typename T>
 static bool wave_grads(const Logits& L) { return L.B * L.S >= kWaveRows && L.V <= kGradSpan<T, 64>; }
 
+// 1024 threads for a row read in one piece: long rows.  In us, 256 threads / 1024: bf16, 8000 rows of 32000 78 / 86, of 50304
+// 121 / 127, of 70000 177 / 166, of 128256 304 / 296; fp32, of 50304 233 / 232, of 70000 341 / 317, of 128256 595 / 584.
+static bool long_rows(const Logits& L) { return L.V > 60000; }
+// Few rows: 1024 threads a row in one launch rather than pieces and a second launch to join them,
+// unless the row is too long for that.  Pieces / one, bf16: 64 rows of 16000 5.1 / 4.3 us, of 50304 6.3 / 6.6 (with the
+// host 8.8 / 6.7), of 128256 7.9 / 11.2; 256 rows of 50304 8.9 / 7.4, of 128256 13.4 / 12.7.
+static bool in_one_piece(int64_t N, int64_t V) { return lse_shape(N, V).pieces == 1 || V <= 65536 || N >= 256; }
+// The losses' terms by row, in the rows' own kernel, and added up by one workgroup: few rows, where a launch less counts (a
+// pass over pairs of 132 rows of 50257 62 -> 56.5 us, policy of 64 rows of 1003 64 -> 57.7).  With many the sums cost more than
+// the launch: pairs of 24000 rows of 1000 28.0 us in two kernels, 23.7 in three.
+constexpr int64_t kTermRows = 4096;
+static bool terms_by_row(int64_t N, int64_t V) { return in_one_piece(N, V) && N <= kTermRows; }
+
+template <typename T, int NT, Then THEN>
+static void launch_lse(const Logits& L, const Scale& c, int pieces, int span, RowSum* part, double inv_temp,
+                       const PolicyArgs& a, float* logp, void* rows, void* seg, hipStream_t st) {
+  const int64_t groups = L.B * L.S * pieces;
+  hipLaunchKernelGGL((lse_partial_kernel<T, NT, THEN>), dim3((unsigned)((groups + kRows<NT> - 1) / kRows<NT>)),
+                     dim3(NT * kRows<NT>), 0, st, L, c, pieces, span, part, inv_temp, a, logp, (RowState*)rows, seg);
+}
+
 template <typename T>
 static hipError_t lse_partial(const Logits& L, const Scale& c, const LseShape& sh, RowSum* part, hipStream_t st) {
-  const int64_t N = L.B * L.S;
-  if (wave_sums<T>(L))
-    hipLaunchKernelGGL((lse_partial_kernel<T, 64, false>), dim3((unsigned)((N + 3) / 4)), dim3(kLseThreads), 0, st, L, c,
-                       sh.pieces, sh.span, part, 0.0, nullptr, nullptr);
-  else
-    hipLaunchKernelGGL((lse_partial_kernel<T, kLseThreads, false>), dim3((unsigned)(N * sh.pieces)), dim3(kLseThreads), 0,
-                       st, L, c, sh.pieces, sh.span, part, 0.0, nullptr, nullptr);
+  const PolicyArgs a{};
+  if (wave_sums<T>(L)) launch_lse<T, 64, kPieces>(L, c, 1, sh.span, part, 0.0, a, nullptr, nullptr, nullptr, st);
+  else if (sh.pieces == 1 && long_rows(L))
+    launch_lse<T, kLongThreads, kPieces>(L, c, 1, sh.span, part, 0.0, a, nullptr, nullptr, nullptr, st);
+  else launch_lse<T, kLseThreads, kPieces>(L, c, sh.pieces, sh.span, part, 0.0, a, nullptr, nullptr, nullptr, st);
+  return hipGetLastError();
+}
+
+// Rows in one piece with what follows for each
+template <typename T, Then THEN>
+static hipError_t lse_then(const Logits& L, const Scale& c, const LseShape& sh, double inv_temp, const PolicyArgs& a,
+                           float* logp, void* rows, void* seg, hipStream_t st) {
+  const int all = (int)L.V;
+  if (wave_sums<T>(L)) launch_lse<T, 64, THEN>(L, c, 1, all, nullptr, inv_temp, a, logp, rows, seg, st);
+  else if (sh.pieces > 1 || long_rows(L))
+    launch_lse<T, kLongThreads, THEN>(L, c, 1, all, nullptr, inv_temp, a, logp, rows, seg, st);
+  else launch_lse<T, kLseThreads, THEN>(L, c, 1, all, nullptr, inv_temp, a, logp, rows, seg, st);
   return hipGetLastError();
 }
 
@@ -822,7 +896,10 @@ int dta_pref_fits(int64_t N, int64_t V) {
   return N >= 0 && V > 0 && N <= kMostGroups && V < ((int64_t)1 << 28) && N * spans < ((int64_t)1 << 31);
 }
 int64_t dta_pref_parts(int64_t N, int64_t V) { return N * lse_shape(N, V).pieces; }
-int64_t dta_pref_segs(int64_t B, int64_t S, int64_t V) { return B * segments(S, lse_shape(B * S, V)); }
+static int segs_of(int64_t B, int64_t S, int64_t V) {
+  return (int)(terms_by_row(B * S, V) ? S : segments(S, lse_shape(B * S, V)));
+}
+int64_t dta_pref_segs(int64_t B, int64_t S, int64_t V) { return B * segs_of(B, S, V); }
 
 hipError_t dta_pref_logprobs(const PrefLogits& l, int type, double temperature, void* part, float* logp, void* rows,
                              hipStream_t st) {
@@ -832,17 +909,11 @@ hipError_t dta_pref_logprobs(const PrefLogits& l, int type, double temperature, 
   const LseShape sh = lse_shape(N, L.V);
   const Scale c = scale_of(temperature);
   DTA_BY_TYPE(type, {
-    if (wave_sums<T>(L)) {
-      hipLaunchKernelGGL((lse_partial_kernel<T, 64, true>), dim3((unsigned)((N + 3) / 4)), dim3(kLseThreads), 0, st, L, c,
-                         1, sh.span, nullptr, 1.0 / temperature, logp, (RowState*)rows);
-    } else if (sh.pieces == 1) {
-      hipLaunchKernelGGL((lse_partial_kernel<T, kLseThreads, true>), dim3((unsigned)N), dim3(kLseThreads), 0, st, L, c, 1,
-                         sh.span, nullptr, 1.0 / temperature, logp, (RowState*)rows);
-    } else {
-      DTA_HIP_CHECK(lse_partial<T>(L, c, sh, (RowSum*)part, st));
-      hipLaunchKernelGGL(logprob_rows_kernel<T>, dim3((unsigned)((N * sh.lanes + 255) / 256)), dim3(256), 0, st, L,
-                         (RowSum*)part, sh.pieces, sh.lanes, c, 1.0 / temperature, logp, (RowState*)rows);
-    }
+    const double inv = 1.0 / temperature;
+    if (in_one_piece(N, L.V)) return lse_then<T, kLogprobs>(L, c, sh, inv, PolicyArgs{}, logp, rows, nullptr, st);
+    DTA_HIP_CHECK(lse_partial<T>(L, c, sh, (RowSum*)part, st));
+    hipLaunchKernelGGL(logprob_rows_kernel<T>, dim3((unsigned)((N * sh.lanes + 255) / 256)), dim3(256), 0, st, L,
+                       (RowSum*)part, sh.pieces, sh.lanes, c, inv, logp, (RowState*)rows);
   })
   return hipGetLastError();
 }
@@ -857,18 +928,22 @@ hipError_t dta_pref_policy(const PrefLogits& l, int type, double temperature, co
   const Logits L = logits_of(l);
   const int64_t N = L.B * L.S;
   const LseShape sh = lse_shape(N, L.V);
-  const int segs = (int)segments(L.S, sh);
+  const int segs = segs_of(L.B, L.S, L.V);
   if (N > 0) {
     const Scale c = scale_of(temperature);
     DTA_BY_TYPE(type, {
-      DTA_HIP_CHECK(lse_partial<T>(L, c, sh, (RowSum*)part, st));
-      hipLaunchKernelGGL(policy_rows_kernel<T>, dim3((unsigned)(L.B * segs)), dim3(256), 0, st, L, (RowSum*)part,
-                         sh.pieces, sh.lanes, c, 1.0 / temperature, policy_args(p), segs, logp, (RowState*)rows,
-                         (double4*)seg);
+      if (terms_by_row(N, L.V)) {
+        DTA_HIP_CHECK((lse_then<T, kPolicy>(L, c, sh, 1.0 / temperature, policy_args(p), logp, rows, seg, st)));
+      } else {
+        DTA_HIP_CHECK(lse_partial<T>(L, c, sh, (RowSum*)part, st));
+        hipLaunchKernelGGL(policy_rows_kernel<T>, dim3((unsigned)(L.B * segs)), dim3(256), 0, st, L, (RowSum*)part,
+                           sh.pieces, sh.lanes, c, 1.0 / temperature, policy_args(p), segs, logp, (RowState*)rows,
+                           (double4*)seg);
+      }
     })
     DTA_HIP_CHECK(hipGetLastError());
   }
-  hipLaunchKernelGGL(policy_total_kernel, dim3(1), dim3(256), 0, st, seg, L.B, segs, p.by_sequence, p.scale,
+  hipLaunchKernelGGL(policy_total_kernel, dim3(1), dim3(kTotalThreads), 0, st, seg, L.B, segs, p.by_sequence, p.scale,
                      loss, stats, weight);
   return hipGetLastError();
 }
@@ -935,17 +1010,21 @@ hipError_t dta_pref_pairs(const PrefLogits& l, int type, const float* ref, int64
   const Logits L = logits_of(l);
   const int64_t N = L.B * L.S;
   const LseShape sh = lse_shape(N, L.V);
-  const int segs = (int)segments(L.S, sh);
+  const int segs = segs_of(L.B, L.S, L.V);
   if (N > 0) {
     const Scale c = scale_of(1.0);
     DTA_BY_TYPE(type, {
-      DTA_HIP_CHECK(lse_partial<T>(L, c, sh, (RowSum*)part, st));
-      hipLaunchKernelGGL(pair_rows_kernel<T>, dim3((unsigned)(L.B * segs)), dim3(256), 0, st, L, (RowSum*)part,
-                         sh.pieces, sh.lanes, c, segs, (RowState*)rows, (double2*)seg);
+      if (terms_by_row(N, L.V)) {
+        DTA_HIP_CHECK((lse_then<T, kPairs>(L, c, sh, 1.0, PolicyArgs{}, nullptr, rows, seg, st)));
+      } else {
+        DTA_HIP_CHECK(lse_partial<T>(L, c, sh, (RowSum*)part, st));
+        hipLaunchKernelGGL(pair_rows_kernel<T>, dim3((unsigned)(L.B * segs)), dim3(256), 0, st, L, (RowSum*)part,
+                           sh.pieces, sh.lanes, c, segs, (RowState*)rows, (double2*)seg);
+      }
     })
     DTA_HIP_CHECK(hipGetLastError());
   }
-  hipLaunchKernelGGL(pair_total_kernel, dim3(1), dim3(256), 0, st, seg, L.B / 2, segs, ref, ref_stride, beta, smoothing,
+  hipLaunchKernelGGL(pair_total_kernel, dim3(1), dim3(kTotalThreads), 0, st, seg, L.B / 2, segs, ref, ref_stride, beta, smoothing,
                      average, scale, (double2*)seg + L.B * segs, loss, logp, margin, weight);
   return hipGetLastError();
 }

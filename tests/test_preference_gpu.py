@@ -517,6 +517,23 @@ def test_short_rows(V, dtype):
     test_preference_loss(2, 1001, V, dtype, 0.1, True, False)
 
 
+@pytest.mark.parametrize("S,V", [(1, 40), (16, 513), (17, 40), (40, 8193), (300, 65)])
+@pytest.mark.parametrize("B", [1, 2, 3, 5, 12, 15, 16, 17, 40])
+def test_sums_over_sequences(B, S, V):
+    """Terms by row, added up by waves: sequences shorter and longer than a thread takes, fewer and more than the waves."""
+    test_policy_loss_without_gradient(B, S, V)
+    test_policy_loss(B, S, V, torch.bfloat16, 0.1, 0.28, "sequence", 0.25)
+    if B % 2 == 0:
+        test_preference_loss(B, S, V, torch.float32, 0.1, True, False)
+
+
+def test_more_rows_than_terms_by_row():
+    for B, S in ((2, 2048), (2, 2049), (128, 32), (2, 33000), (4100, 2), (1, 70001)):
+        test_policy_loss_without_gradient(B, S, 9)
+        if B % 2 == 0:
+            test_preference_loss(B, S, 9, torch.bfloat16, 0.0, False, True)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V", [900, 2000, 4000])
 def test_extreme_logits_in_short_rows(V, dtype):
