@@ -694,8 +694,8 @@ __device__ __forceinline__ void add_chunks(Chunk<T> (&r)[N], int V, const Scale&
 
 // One workgroup a row, the row in registers between its two uses (NT * CHUNKS chunks, at least the row's): one read and
 // one write of the logits' size.  It ran at 4.6-5.1 TB/s until less arithmetic
-// and fewer registers a row brought 5.6-5.9 of the copy's 6.1; what is left is the time that a row's terms keep its
-// workgroup waiting.
+// and fewer registers a row brought 5.5-5.9 of the copy's 6.1 (8192 x 50304 bf16, 3/4 of the rows counting: 260 us); what is
+// left is mostly the time that a row's terms keep its workgroup waiting.
 template <typename T, int NT, int CHUNKS, int WAVES>  // WAVES a SIMD that the registers leave room for
 __global__ void __launch_bounds__(NT * kRows<NT>, WAVES) policy_fused_kernel(Logits L, Scale c, double inv_temp, PolicyArgs a,
                                                                  const float* __restrict__ weight,
