@@ -128,9 +128,6 @@ int64_t weight_at(int64_t N) { return (16 * N + 255) / 256 * 256; }
 
 void logits_grad(const Tensor& z, const Tensor& target, const Tensor& state, bool weighted, const Tensor& g,
                  int64_t ignore, double temperature, bool unless_one, const Tensor& dz) {
-  // (a second derivative would need more than this formula: refused rather than silently wrong)
-  TORCH_CHECK(!(torch::GradMode::is_enabled() && g.requires_grad()),
-              "the preference losses can be differentiated once: no create_graph through them");
   int type;
   const auto l = logits_arg(z, target, ignore, &type);
   const Tensor gf = g.scalar_type() == torch::kFloat32 ? g : g.to(torch::kFloat32);
@@ -141,6 +138,18 @@ void logits_grad(const Tensor& z, const Tensor& target, const Tensor& state, boo
   ok(dta_pref_grad(l, type, temperature, s, weighted ? reinterpret_cast<float*>(s + weight_at(l.B * l.S)) : nullptr,
                    gout, unless_one, dz.data_ptr(), stream_on(z)),
      "logits gradient");
+}
+
+// A backward under create_graph: its gradient stands in the graph behind the logits and the gradient that arrived, so that
+// whoever differentiates it again (by way of either) is refused, not handed a result that lacks a term
+struct DifferentiatedOnce : torch::autograd::Function<DifferentiatedOnce> {
+  static Tensor forward(AutogradContext*, const Tensor& dz, const Tensor&, const Tensor&) { return dz.detach(); }
+  static variable_list backward(AutogradContext*, const variable_list&) {
+    TORCH_CHECK(false, "the preference losses can be differentiated once: no second derivative through them");
+  }
+};
+Tensor once(const Tensor& dz, const Tensor& z, const Tensor& g) {
+  return torch::GradMode::is_enabled() ? DifferentiatedOnce::apply(dz, z, g) : dz;
 }
 
 struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
@@ -168,7 +177,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     Tensor dz = torch::empty(z.sizes(), z.options());
     logits_grad(z, target, saved[2], false, grads[0], ctx->saved_data["ignore"].toInt(),
                 ctx->saved_data["temperature"].toDouble(), false, dz);
-    return {dz, Tensor(), Tensor(), Tensor()};
+    return {once(dz, z, grads[0]), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -241,7 +250,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     if (!written) dz = torch::empty(z.sizes(), z.options());
     logits_grad(z, target, saved[2], true, grads[0], data["ignore"].toInt(), data["temperature"].toDouble(), written,
                 dz);
-    none[0] = dz;
+    none[0] = once(dz, z, grads[0]);
     return none;
   }
 };
@@ -291,7 +300,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     const at::DeviceGuard guard(saved[0].device());
     Tensor dz = torch::empty(saved[0].sizes(), saved[0].options());
     logits_grad(saved[0], saved[1], saved[2], true, grads[0], ctx->saved_data["ignore"].toInt(), 1.0, false, dz);
-    none[0] = dz;
+    none[0] = once(dz, saved[0], grads[0]);
     return none;
   }
 };

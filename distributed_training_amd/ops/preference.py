@@ -9,7 +9,8 @@ a position does not count (prompts, padding).  Positions that do not count -- a 
 GPU tensors take the HIP kernels of ``csrc/preference.hip`` (bf16, fp16 or fp32 logits; rows of any stride and
 alignment, any vocabulary) through the autograd functions of ``csrc/bindings_pref.cpp``, which check their tensors.
 CPU tensors take the same math in PyTorch.  Per-token inputs are fp32; statistics over the vocabulary are fp32,
-per-token terms and sums fp64.  Each loss can be differentiated once.
+per-token terms and sums fp64.  On the GPU each loss can be differentiated once: a gradient taken with ``create_graph`` is
+refused where it is differentiated itself.
 """
 from __future__ import annotations
 

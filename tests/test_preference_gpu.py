@@ -570,3 +570,32 @@ def test_extreme_logits_in_short_rows(V, dtype):
     assert (near | (lp[:40] == lp_few))[live].all()
     tol = g_few.double().abs() * (2 * oracle.half_step(dtype) * 1.01 + 2 * e) + oracle.smallest(dtype) * 2
     assert ((g[:40].double() - g_few.double()).abs() <= tol + 2 * e / 0.7)[live].all()
+
+
+@pytest.mark.parametrize("S", [6, 150])  # few rows, and enough for the policy loss's one-pass form
+@pytest.mark.parametrize("which", ["logprobs", "policy", "preference"])
+def test_second_derivatives_are_refused(which, S):
+    """A gradient taken with create_graph is right as it is; whoever differentiates it is told, through whichever of its
+    inputs, and nothing that lacks the gradient's own term comes back."""
+    z, target, old, ref, adv = _case(4, S, 203, torch.float32)
+    loss_of = {"logprobs": lambda x: preference.token_logprobs(x, target).mean(),
+               "policy": lambda x: preference.policy_loss(x, target, old, adv, ref, kl_coef=0.1).loss,
+               "preference": lambda x: preference.preference_loss(x, target).loss}[which]
+    leaf = z.clone().requires_grad_()
+    (want,) = torch.autograd.grad(loss_of(leaf), leaf)
+    loss = loss_of(leaf)
+    (g,) = torch.autograd.grad(loss, leaf, create_graph=True)
+    assert torch.equal(g.detach(), want)
+    with pytest.raises(RuntimeError, match="differentiated once"):  # the loss and a penalty on its gradient
+        (loss + g.square().sum()).backward()
+    half = torch.full((), 0.5, device=DEV, requires_grad=True)
+    for inputs in ([leaf], [half], [leaf, half]):  # by way of logits that are computed, and of the gradient that arrived
+        loss = loss_of(leaf * 2.0) * half
+        (g,) = torch.autograd.grad(loss, leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            torch.autograd.grad(g.square().sum(), inputs)
+    # a penalty on a gradient that does not come through the losses
+    w = torch.full((), 3.0, device=DEV, requires_grad=True)
+    (gw,) = torch.autograd.grad(loss_of(leaf) + w ** 3, w, create_graph=True)
+    gw.square().backward()
+    assert float(w.grad) == 2 * 27.0 * 18.0
