@@ -599,3 +599,63 @@ def test_second_derivatives_are_refused(which, S):
     (gw,) = torch.autograd.grad(loss_of(leaf) + w ** 3, w, create_graph=True)
     gw.square().backward()
     assert float(w.grad) == 2 * 27.0 * 18.0
+
+
+def _policy_forward_near(B, S, V, dtype):
+    """The forward alone against the definition (test_policy_loss has the gradient's form, which may be another)."""
+    z, target, old, ref, adv = _case(B, S, V, dtype, seed=B + S + V)
+    with torch.no_grad():
+        out = preference.policy_loss(z, target, old, adv, ref, kl_coef=0.1)
+    loss, lp, mean_kl, clipped = oracle.policy64(z.double(), target, old, adv, ref, kl_coef=0.1)
+    live = (target != -100).double()
+    n = live.sum().clamp(min=1)
+    e = oracle.stat_error(z.double())
+    d = torch.where(live > 0, ref.double() - lp, torch.zeros_like(lp))
+    # d/dlp of a token's term is at most r |A| + kl |expm1(d)|, of its KL |expm1(d)|; the second order in e behind it
+    steep = (torch.exp(lp - old.double()) * adv.double().abs() + 0.1 * torch.expm1(d).abs() + e) * live / n
+    assert abs(float(out.loss) - float(loss)) <= float(steep.sum()) * e * 1.01 + abs(float(loss)) * 2.0 ** -24
+    assert ((out.logp.double() - lp).abs() <= e + lp.abs() * 2.0 ** -24).all()
+    kl_tol = float(((torch.expm1(d).abs() + e) * live * e).sum() / n) * 1.01 + abs(float(mean_kl)) * 2.0 ** -24
+    assert abs(float(out.kl) - float(mean_kl)) <= kl_tol
+    assert abs(float(out.clip_fraction) - float(clipped)) <= 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,S,V", [(1, 3, 70001), (2, 20, 128251), (4, 10, 65543), (2, 127, 70001), (3, 85, 70001), (2, 1, 600001)])
+def test_rows_in_pieces(B, S, V, dtype):
+    """Under 256 rows of more than 65536 logits are cut into pieces: odd vocabularies (a remainder behind the last piece's whole
+    chunks), 8 to 64 lanes a row in the kernels that join them, sequences over several of their workgroups."""
+    test_token_logprobs(B, S, V, dtype, 0.7)
+    test_policy_loss(B, S, V, dtype, 0.1, 0.28, "sequence", 0.25)
+    _policy_forward_near(B, S, V, dtype)
+    if B % 2 == 0:
+        test_preference_loss(B, S, V, dtype, 0.1, True, False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_extreme_logits_in_pieces(dtype):
+    test_extreme_logits(70001, dtype, 0.7)
+    V = 70001  # nine pieces of 7784 logits
+    z = torch.full((1, 5, V), float("-inf"), device=DEV, dtype=dtype)
+    target = torch.full((1, 5), V - 1, device=DEV)
+    z[0, 0, V - 1] = 3.0  # one logit, behind the last whole chunk
+    z[0, 1, 7784 * 4], z[0, 1, V - 1] = 1.0, 1.0  # a piece of one logit between pieces of none
+    z[0, 2, 5], z[0, 3, 60000] = float("nan"), float("inf")
+    z.requires_grad_()
+    lp = preference.token_logprobs(z, target)
+    (grad,) = torch.autograd.grad(lp.sum(), z)
+    lp = lp.detach()
+    assert float(lp[0, 0]) == 0.0 and abs(float(lp[0, 1]) + math.log(2.0)) < 2.0 ** -20
+    assert torch.isnan(lp[0, 2:]).all() and torch.isnan(grad[0, 2:]).any(-1).all()
+    assert not grad[0, 0].any()
+    # p = 1/2 with an error of stat_error's order in its exponent (reach 17 for V = 70001: under 2^-16), half a step of the type
+    for j, want in ((7784 * 4, -0.5), (V - 1, 0.5)):
+        assert abs(float(grad[0, 1, j]) - want) <= 0.5 * (oracle.half_step(dtype) + 2.0 ** -16)
+    assert int(torch.count_nonzero(grad[0, 1])) == 2
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_long_rows_by_the_thousand(dtype):
+    """More rows than their terms are added up one by one, each of 1024 threads."""
+    _policy_forward_near(2, 2050, 60001, dtype)
+    test_preference_loss(2, 2050, 60001, dtype, 0.1, True, False)
