@@ -822,7 +822,8 @@ static bool wave_grads(const Logits& L) { return L.B * L.S >= kWaveRows && L.V <
 
 // 1024 threads for a row read in one piece: long rows.  In us, 256 threads / 1024: bf16, 8000 rows of 32000 78 / 86, of 50304
 // 121 / 127, of 70000 177 / 166, of 128256 304 / 296; fp32, of 50304 233 / 232, of 70000 341 / 317, of 128256 595 / 584.
-static bool long_rows(const Logits& L) { return L.V > 60000; }
+// (Of 2^22 rows and more 256 again: a launch takes fewer than 2^32 threads.)
+static bool long_rows(const Logits& L) { return L.V > 60000 && L.B * L.S < (1 << 22); }
 // Few rows: 1024 threads a row in one launch rather than pieces and a second launch to join them,
 // unless the row is too long for that.  Pieces / one, bf16: 64 rows of 16000 5.1 / 4.3 us, of 50304 6.3 / 6.6 (with the
 // host 8.8 / 6.7), of 128256 7.9 / 11.2; 256 rows of 50304 8.9 / 7.4, of 128256 13.4 / 12.7.
@@ -889,7 +890,8 @@ static TokenArray array_of(const PrefTokens& t) { return {t.p, t.sb, t.ss}; }
     default: return hipErrorInvalidValue;             \
   }
 
-// A launch takes fewer than 2^32 threads, and the row passes give a row a workgroup of 256; units are counted in 32 bits
+// A launch takes fewer than 2^32 threads, and the row passes give a row a workgroup of 256 (1024 only to fewer than 2^22
+// rows); units are counted in 32 bits
 constexpr int64_t kMostGroups = ((int64_t)1 << 24) - 1;
 int dta_pref_fits(int64_t N, int64_t V) {
   const int64_t spans = (V + kGradSpan<float> - 1) / kGradSpan<float>;

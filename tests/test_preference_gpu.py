@@ -659,3 +659,28 @@ def test_long_rows_by_the_thousand(dtype):
     """More rows than their terms are added up one by one, each of 1024 threads."""
     _policy_forward_near(2, 2050, 60001, dtype)
     test_preference_loss(2, 2050, 60001, dtype, 0.1, True, False)
+
+
+def test_rows_beyond_a_launch_of_wide_workgroups():
+    """2^22 rows of a long vocabulary (expanded logits: no memory behind them): with 1024 threads a row the launch would take
+    2^32, so these get 256.  All but a few positions are ignored, and those are as the definition says."""
+    B, S, V = 2, 2 ** 21, 60001
+    base = torch.randn(V, generator=torch.Generator().manual_seed(0)).bfloat16().to(DEV)
+    z = base.expand(B, S, V)
+    target = torch.full((B, S), -100, device=DEV)
+    at = torch.tensor([0, 1, S // 2, S - 1], device=DEV)
+    target[:, at] = torch.tensor([[5, V - 1, 70, 0], [9, 9, V - 2, 1]], device=DEV)
+    few = target[:, at]
+    want, _ = oracle.logprobs64(base.double().expand(B, 4, V), few)
+    e = oracle.stat_error(base.double()[None])
+    lp = preference.token_logprobs(z, target)
+    assert ((lp[:, at].double() - want).abs() <= e + want.abs() * 2.0 ** -24).all()
+    lp[:, at] = 0.0
+    assert not lp.any()
+    zero, one = torch.zeros(B, S, device=DEV), torch.ones(B, device=DEV)
+    out = preference.policy_loss(z, target, zero, one)
+    r = want.exp()  # at most 1: unclipped, or clipped from below where the advantage is positive: -r A either way
+    assert abs(float(out.loss) + float(r.mean())) <= float(r.mean()) * (e + 2.0 ** -24) * 1.01
+    pair = preference.preference_loss(z, target, average=True)
+    L = want.mean(1)
+    assert ((pair.logp.double() - L).abs() <= e + L.abs() * 2.0 ** -24).all()
