@@ -202,9 +202,11 @@ def clip_flat_grad_norm_(fg: FlatParamGroup, max_norm: float, comm: Any = None, 
     """Global-norm gradient clipping over ONE flat gradient buffer (what
     ``torch.nn.utils.clip_grad_norm_`` computes over the module's parameters).
 
-    ``sharded``: the buffer holds this rank's shard only (FSDP), so the squared
-    norm is all-reduced (sum) over ``comm`` before the coefficient is formed --
-    every rank then scales its shard by the SAME coefficient.  Replicated
+    ``sharded``: the buffer holds this rank's shard only (FSDP), so the ranks' sums of
+    squares are gathered over ``comm`` and added in 64 bits, in the ranks' order, before
+    the coefficient is formed -- every rank then scales its shard by the SAME coefficient,
+    also where the squares leave fp32's range.  (Gathered, not all-reduced: every
+    communicator gathers any type, the node-local one reduces no fp64.)  Replicated
     buffers (DDP after the all-reduce) need no collective.  No host sync: the
     coefficient stays on the device.  Padding between parameters is zero and
     does not change the norm.  Returns the total norm (0-dim tensor)."""
@@ -215,17 +217,14 @@ def clip_flat_grad_norm_(fg: FlatParamGroup, max_norm: float, comm: Any = None, 
     g = fg.grad
     if not (sharded and comm is not None and comm.world_size > 1):
         return clip_grads_([g], max_norm).reshape(())
-    sq = grad_sumsq([g])[0].float().reshape(1)
-    dev = getattr(comm, "device", None)
-    if dev is not None and sq.device != torch.device(dev):  # host-resident shards, device communicator
-        sq_d = sq.to(dev)
-        comm.all_reduce(sq_d, op="sum")
-        sq = sq_d.to(sq.device)
-    else:
-        comm.all_reduce(sq, op="sum")
-    sq = sq.reshape(())
-    grad_clip_([g], sq.double(), max_norm)
-    return sq.sqrt()
+    # twice each: 16 bytes a rank, what the node-local gather moves without staging
+    dev = torch.device(getattr(comm, "device", None) or g.device)  # (host-resident shards: a device communicator's)
+    sq = grad_sumsq([g])[0].expand(2).contiguous().to(dev)
+    every = torch.empty(comm.world_size * 2, dtype=sq.dtype, device=dev)
+    comm.all_gather_into(every, sq)
+    total = every[::2].sum().to(g.device)
+    grad_clip_([g], total, max_norm)
+    return total.sqrt().float()
 
 
 def plan_buckets(numels: Sequence[int], esize: int, cap_bytes: int, first_cap_bytes: int) -> List[List[int]]:

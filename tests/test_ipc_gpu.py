@@ -119,6 +119,33 @@ def test_ipc_collectives_shared_gpu(ws):
     run_gloo(_coll_worker, ws, 0.25)  # 256 KiB slots: multi-segment messages
 
 
+def _clip_worker(rank, ws):
+    """FSDP's clip over shards, with the node-local communicator: the squares are added in 64 bits across the ranks."""
+    from types import SimpleNamespace
+
+    from distributed_training_amd.parallel.flat import clip_flat_grad_norm_
+    from distributed_training_amd.parallel.ipc import IpcComm
+
+    dev = _shared()
+    comm = IpcComm(rank, ws, dev)
+    for scale in (1e25, 1.0, 1e-30):
+        shards = [torch.linspace(-1, 2, 100003 + 7 * r) * scale for r in range(ws)]
+        want = torch.cat(shards).double().square().sum().sqrt()
+        g = shards[rank].to(dev)
+        fg = SimpleNamespace(grad=g, prepare_grads_for_step=lambda: True)
+        norm = clip_flat_grad_norm_(fg, 0.25, comm=comm, sharded=True)
+        torch.cuda.synchronize()
+        torch.testing.assert_close(norm.cpu().double(), want, rtol=2.0 ** -23, atol=0)
+        after = shards[rank].double() * (0.25 / (want + 1e-6)).clamp(max=1.0)
+        torch.testing.assert_close(g.cpu().double(), after, rtol=2.0 ** -22, atol=2.0 ** -149)
+    comm.poll_errors()
+    comm.destroy()
+
+
+def test_clip_of_shards_in_64_bits_shared_gpu():
+    run_gloo(_clip_worker, 2)
+
+
 def _bf16_8rank_worker(rank, ws):
     """bf16 all-reduce at 8 ranks: ONE rounding of the exact fp32 rank-order sum."""
     from distributed_training_amd.parallel.ipc import IpcComm

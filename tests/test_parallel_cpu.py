@@ -207,6 +207,39 @@ def test_clip_grad_norm_global(strategy):
     run_gloo(_clip_parity, 2, strategy)
 
 
+def _clip_range(rank, ws):
+    """Gradients whose squares leave fp32's range, of nothing, and non-finite ones: the norm over the ranks' shards."""
+    from types import SimpleNamespace
+
+    from distributed_training_amd.parallel.comm import TorchComm
+    from distributed_training_amd.parallel.flat import clip_flat_grad_norm_
+
+    comm = TorchComm()
+    for scale in (1e25, 1e-30, 1.0, 0.0, float("inf"), float("nan")):
+        shards = [torch.linspace(-1, 2, 1000 + 7 * r) for r in range(ws)]
+        shards[1] *= scale if scale == scale and abs(scale) != float("inf") else 1.0
+        if scale != scale or abs(scale) == float("inf"):
+            shards[1][3] = scale
+        elif scale > 1 or scale == 1e-30:  # every rank's shard, rank 0's the smaller or the larger part
+            shards[0] *= scale * 0.5
+        want = torch.cat(shards).double().square().sum().sqrt()
+        g = shards[rank].clone()
+        fg = SimpleNamespace(grad=g, prepare_grads_for_step=lambda: True)
+        norm = clip_flat_grad_norm_(fg, 0.25, comm=comm, sharded=True)
+        assert norm.shape == () and norm.dtype == torch.float32
+        torch.testing.assert_close(norm.double(), want, rtol=2.0 ** -23, atol=0, equal_nan=True)
+        after = shards[rank].double() * (0.25 / (want + 1e-6)).clamp(max=1.0)
+        # the coefficient and the product in fp32
+        torch.testing.assert_close(g.double(), after, rtol=2.0 ** -22, atol=2.0 ** -149, equal_nan=True)
+        same = [torch.empty(()) for _ in range(ws)]
+        dist.all_gather(same, norm)
+        assert all(torch.equal(s, norm) or norm != norm for s in same)
+
+
+def test_clip_of_shards_in_64_bits():
+    run_gloo(_clip_range, 2)
+
+
 def _comm_ops(rank, ws):
     from distributed_training_amd.parallel.comm import TorchComm
 
