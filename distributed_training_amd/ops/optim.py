@@ -43,13 +43,17 @@ def _fills_memory(t: torch.Tensor) -> bool:
 
 
 def _by_device(tensors: Iterable[torch.Tensor]) -> Dict[torch.device, List[torch.Tensor]]:
-    """The tensors by device; sparse and non-floating ones are refused."""
+    """The tensors by device, complex ones as the real and imaginary parts that they hold (``|z|^2`` is the sum of
+    their squares); sparse and non-floating ones are refused."""
     found: Dict[torch.device, List[torch.Tensor]] = {}
     for t in tensors:
+        t = t.detach()
+        if t.is_complex() and t.layout == torch.strided:  # (a conjugate view's memory holds the same squares)
+            t = torch.view_as_real(t.conj() if t.is_conj() else t)
         if t.layout != torch.strided or not t.dtype.is_floating_point or t.element_size() == 1:
-            raise TypeError(f"gradient norm: dense float64, float32, bfloat16 or float16 tensors (got {t.dtype}, "
-                            f"{t.layout})")
-        found.setdefault(t.device, []).append(t.detach())
+            raise TypeError(f"gradient norm: dense float64, float32, bfloat16 or float16 tensors, or complex ones of "
+                            f"these (got {t.dtype}, {t.layout})")
+        found.setdefault(t.device, []).append(t)
     return found
 
 
@@ -99,7 +103,7 @@ def grad_clip_(tensors: Iterable[torch.Tensor], sumsq: torch.Tensor, max_norm: f
 
 def global_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]]) -> torch.Tensor:
     """The 2-norm over all elements of all tensors: a 0-dim fp32 tensor (0 where there are none).  Any mix of sizes
-    and of fp64 / fp32 / bf16 / fp16."""
+    and of fp64 / fp32 / bf16 / fp16, complex numbers counting with their modulus."""
     return grad_sumsq([tensors] if isinstance(tensors, torch.Tensor) else tensors)[1]
 
 
@@ -124,7 +128,8 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scale the parameters' gradients in place so that their global 2-norm is at most ``max_norm``, and return the
     norm before (a 0-dim fp32 tensor).  As ``torch.nn.utils.clip_grad_norm_`` with its 2-norm: the coefficient is
-    ``min(1, max_norm / (norm + 1e-6))``, a NaN norm makes every gradient NaN; parameters without a gradient are
+    ``min(1, max_norm / (norm + 1e-6))``, a NaN norm makes every gradient NaN; a complex gradient counts with its modulus
+    and keeps its angle; parameters without a gradient are
     skipped, and one that is listed twice (or a gradient that two share) counts and is scaled once; gradients on the
     GPU that share a part of their memory are refused.  On the GPU the norm is one pass over every gradient and the
     scaling another, left out on the device where the norm is within the bound: no host sync unless

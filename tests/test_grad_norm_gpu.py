@@ -229,3 +229,25 @@ def test_gradients_on_the_host_and_the_device():
     norm = optim.clip_grad_norm_([a, b], 1.0)
     assert abs(float(norm) - want) <= 2.0 ** -23 * want
     assert torch.allclose(a.grad.double(), before / want, rtol=1e-6) and torch.allclose(b.grad, torch.full((50,), 2.0 / want), rtol=1e-6)
+
+
+@pytest.mark.parametrize("dtype", [torch.complex64, torch.complex128])
+def test_complex_gradients(dtype):
+    """As their real and imaginary parts: dense, strided and conjugate ones beside real ones."""
+    z = torch.randn(60, 70, dtype=dtype, generator=torch.Generator().manual_seed(0)).to(DEV)
+    wide = z.clone()
+    grads = [z[:, 20:50].contiguous(), wide[:, 1:3], z[:20].clone().conj(), z.real[0].float().contiguous()]
+    before = [g.resolve_conj().clone() for g in grads]
+    norm = math.sqrt(sum(float((b.abs().double() ** 2).sum()) for b in before))
+    params = [torch.nn.Parameter(torch.zeros(g.shape, dtype=g.dtype, device=DEV)) for g in grads]
+    for p, g in zip(params, grads):
+        p.grad = g
+    for flag in (False, True):
+        for g, b in zip(grads, before):
+            g.copy_(b)
+        got = optim.clip_grad_norm_(params + params[:1], 0.5, error_if_nonfinite=flag)
+        # the oracle squares moduli that torch rounds to the parts' type (2 roundings of 2^-24 at most, halved by the root's mean)
+        assert abs(float(got) - norm) <= 2.0 ** -22 * norm
+        for p, b in zip(params, before):
+            torch.testing.assert_close(p.grad.resolve_conj(), b * (0.5 / (norm + 1e-6)), rtol=2.0 ** -21, atol=0)
+        assert torch.equal(wide[:, 3:], z[:, 3:]) and torch.equal(wide[:, :1], z[:, :1])

@@ -245,3 +245,60 @@ def test_norm_refusals():
         optim.global_norm([torch.ones(3, dtype=torch.long)])
     with pytest.raises(TypeError, match="gradient norm"):
         optim.global_norm([torch.eye(3).to_sparse()])
+
+
+@pytest.mark.parametrize("dtype", [torch.complex64, torch.complex128])
+def test_clip_of_complex_gradients(dtype):
+    """A complex parameter's gradient counts with its modulus, beside real ones, as torch's clip has it; also a strided one and a
+    conjugate view, of which torch's refuses the latter."""
+    g = torch.Generator().manual_seed(0)
+    z = torch.randn(6, 7, dtype=dtype, generator=g)
+    grads = [z[:, 2:5].clone(), z[:, 1:3], z[:2].clone(), torch.randn(5, generator=g)]
+    params, theirs = [], []
+    for x in grads:
+        for found, grad in ((params, x.clone(memory_format=torch.preserve_format)), (theirs, x.clone())):
+            found.append(torch.nn.Parameter(torch.zeros(x.shape, dtype=x.dtype)))
+            found[-1].grad = grad
+    wide = z.clone()
+    params[1].grad = wide[:, 1:3]  # gaps between its rows
+    params[2].grad = params[2].grad.conj()
+    assert params[2].grad.is_conj()
+    want = torch.nn.utils.clip_grad_norm_(theirs, 0.5)
+    norm = optim.clip_grad_norm_(params + params[:1], 0.5)
+    # torch's fp32 sums: 61 terms and their roots
+    torch.testing.assert_close(norm.double(), want.double(), rtol=64 * 2.0 ** -24, atol=0)
+    for k, (p, q) in enumerate(zip(params, theirs)):
+        grad = p.grad.conj() if k == 2 else p.grad
+        torch.testing.assert_close(grad, q.grad, rtol=64 * 2.0 ** -24, atol=0)
+    assert torch.equal(wide[:, 3:], z[:, 3:]) and torch.equal(wide[:, :1], z[:, :1])
+    with pytest.raises(TypeError, match="gradient norm"):
+        optim.global_norm([z.to_sparse()])
+
+
+def test_the_trainer_clips_complex_gradients():
+    """The trainer's clip over a plain module takes what torch's took."""
+    from types import SimpleNamespace
+
+    from distributed_training_amd.engine.trainer import Trainer
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w = torch.nn.Parameter(torch.ones(3, 2, dtype=torch.complex64) * (1 - 2j))
+            self.b = torch.nn.Parameter(torch.ones(2))
+
+        def forward(self, x):
+            return (x.to(self.w.dtype) @ self.w).abs() + self.b
+
+    x, y = torch.linspace(-1, 1, 12).view(4, 3), torch.zeros(4, 2)
+    nets = Net(), Net()
+    torch.nn.functional.mse_loss(nets[1](x), y).backward()
+    norm = torch.nn.utils.clip_grad_norm_(nets[1].parameters(), 0.1)
+    assert float(norm) > 0.1
+    torch.optim.SGD(nets[1].parameters(), lr=1.0).step()
+    trainer = SimpleNamespace(optimizer=torch.optim.SGD(nets[0].parameters(), lr=1.0), model=nets[0],
+                              config=SimpleNamespace(loss="mse", grad_clip=0.1), _loss_fn=torch.nn.functional.mse_loss)
+    Trainer._run_batch_eager(trainer, x, y)
+    for a, b in zip(nets[0].parameters(), nets[1].parameters()):
+        # torch's fp32 norm of 8 numbers, and the step's own subtraction
+        torch.testing.assert_close(a, b, rtol=16 * 2.0 ** -24, atol=16 * 2.0 ** -24 * 0.1)
