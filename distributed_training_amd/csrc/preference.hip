@@ -329,8 +329,9 @@ struct TokenInputs {
 };
 
 // One token: the loss term, and its slope by lp.  min(r A, clip(r) A) has slope r A except where the clipped term is the
-// smaller one: A > 0 above the upper bound, A < 0 below the lower one.  r = exp(lp - old), q = exp(ref - lp): the KL term
-// q - 1 - d is exact to 2^-52 absolutely, far below what the rounding of ref_logp to fp32 does to it.
+// smaller one: A > 0 above the upper bound, A < 0 below the lower one.  r = exp(lp - old), q = exp(ref - lp).  The KL term
+// q - 1 - d keeps 52 bits below 1, of which a small d leaves few in d^2 / 2: below 2^-7 it is the series' first five terms
+// (the next is d^5 / 2520 of the first: 2^-46), and q - 1 is d more than that.
 __device__ __forceinline__ void policy_token(const PolicyArgs& a, const TokenInputs& in, double lp, double r, double q,
                                              double* loss, double* slope, double* kl, bool* clipped) {
   const double A = (double)in.adv;
@@ -340,8 +341,10 @@ __device__ __forceinline__ void policy_token(const PolicyArgs& a, const TokenInp
   *slope = *clipped ? 0.0 : -r * A;
   *kl = 0.0;
   if (in.has_ref) {
-    const double d = (double)in.ref_logp - lp, e = q - 1.0;
-    *kl = e < d ? 0.0 : e - d;  // (never below 0, rounded or not)
+    const double d = (double)in.ref_logp - lp;
+    const bool small = fabs(d) < 0x1p-7;
+    *kl = small ? d * d * (1.0 / 2 + d * (1.0 / 6 + d * (1.0 / 24 + d * (1.0 / 120 + d * (1.0 / 720))))) : q - 1.0 - d;
+    const double e = small ? d + *kl : q - 1.0;
     if (a.kl_coef != 0.0) {
       *loss += a.kl_coef * *kl;
       *slope -= a.kl_coef * e;
@@ -660,11 +663,10 @@ __global__ void __launch_bounds__(1024) policy_weight_kernel(Logits L, int by_se
   if (threadIdx.x == 0) *count = v[0];
 }
 
-// What a row adds to the loss (times the row's weight), to the mean KL (held in fp32, which the mean is returned in) and to
-// the count of clipped tokens
+// What a row adds to the loss (times the row's weight), and its KL term (never below 0), whose sign says that the token is
+// clipped
 struct PolicyTerms {
-  double loss;
-  float kl, clipped;
+  double loss, kl;
 };
 
 // Running (m, s) of a thread over its chunks of a row
@@ -712,7 +714,7 @@ __global__ void __launch_bounds__(NT * kRows<NT>, WAVES) policy_fused_kernel(Log
     if (tid == 0) {
       logp[row] = 0.f;
       rows[row] = RowState{0.f, 0.f, 0.f, 0.f};
-      terms[row] = {0.0, 0.f, 0.f};
+      terms[row] = {0.0, 0.0};
     }
     return;
   }
@@ -747,7 +749,7 @@ __global__ void __launch_bounds__(NT * kRows<NT>, WAVES) policy_fused_kernel(Log
     if (tid == 0) {
       logp[row] = (float)lp;
       rows[row] = st;
-      terms[row] = {loss * (double)w, (float)kl, clipped ? 1.f : 0.f};
+      terms[row] = {loss * (double)w, copysign(kl, clipped ? -1.0 : 1.0)};
     }
   }
   if constexpr (NT == 64) {  // the wave's first lane has them
@@ -776,8 +778,8 @@ __global__ void __launch_bounds__(1024) policy_sum_kernel(const PolicyTerms* __r
   for (unsigned i = threadIdx.x; i < (unsigned)N; i += 1024) {
     const PolicyTerms x = terms[i];
     v[0] += x.loss;
-    v[1] += (double)x.kl;
-    v[2] += (double)x.clipped;
+    v[1] += fabs(x.kl);
+    v[2] += signbit(x.kl) ? 1.0 : 0.0;
   }
   block_sums64<3, 16>(v);
   if (threadIdx.x == 0) {

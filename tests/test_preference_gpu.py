@@ -684,3 +684,24 @@ def test_rows_beyond_a_launch_of_wide_workgroups():
     pair = preference.preference_loss(z, target, average=True)
     L = want.mean(1)
     assert ((pair.logp.double() - L).abs() <= e + L.abs() * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("S,grad", [(20, True), (20, False), (200, True), (5000, True), (5000, False)])
+@pytest.mark.parametrize("step", [1e-5, -3e-4, 0.0077, 0.0079])
+def test_small_kl(S, grad, step):
+    """A reference next to the policy: exp(d) - 1 - d of a d of 1e-5 and more, in every form of the loss.  Uniform rows, whose
+    log-probability -log V is exact to 64 bits: log2, its product with ln 2 and the oracle's logarithm are within 2^-52 of it each,
+    d within their sum, the KL term within twice that of d (and the series within 2^-46); then one rounding to fp32."""
+    V = 1003
+    z = torch.zeros(1, S, V, device=DEV, requires_grad=grad)
+    target = torch.arange(S, device=DEV).remainder(V)[None]
+    lp = -math.log(V)
+    ref = (lp + step * torch.linspace(0.9, 1.1, S, dtype=torch.float64)).float().to(DEV)[None]
+    d = ref.double() - lp
+    out = preference.policy_loss(z, target, torch.full_like(ref, lp), torch.zeros_like(ref), ref, kl_coef=0.5)
+    # the same series to d^8, far below 2^-53 of it
+    want = d * d * sum(d ** n / math.factorial(n + 2) for n in range(7))
+    tol = 2.0 ** -24 * 1.01 + 2 * 3 * 2.0 ** -52 * abs(lp) / (0.9 * abs(step)) + 2.0 ** -46
+    assert abs(float(out.kl) / float(want.mean()) - 1.0) <= tol
+    assert abs(float(out.loss.detach()) / (0.5 * float(want.mean())) - 1.0) <= tol + 2.0 ** -24
+    assert float(out.clip_fraction) == 0.0
