@@ -135,7 +135,7 @@ void logits_grad(const Tensor& z, const Tensor& target, const Tensor& state, boo
                                              : tokens_arg(gf, target, "gradient");
   TORCH_CHECK(gf.device() == z.device(), "gradient is on ", gf.device(), ", logits on ", z.device());
   char* s = static_cast<char*>(state.data_ptr());
-  ok(dta_pref_grad(l, type, temperature, s, weighted ? reinterpret_cast<float*>(s + weight_at(l.B * l.S)) : nullptr,
+  ok(dta_pref_grad(l, type, temperature, s, weighted ? reinterpret_cast<double*>(s + weight_at(l.B * l.S)) : nullptr,
                    gout, unless_one, dz.data_ptr(), stream_on(z)),
      "logits gradient");
 }
@@ -202,7 +202,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     const int64_t N = l.B * l.S;
     const bool fused = grad && dta_pref_policy_fused(type, N, l.V);
     Arena a;
-    const int64_t rows = a.add(16 * N), weight = a.add(4 * l.B);
+    const int64_t rows = a.add(16 * N), weight = a.add(8 * l.B);
     const int64_t part = a.add(fused ? 16 * N + 8 : 16 * dta_pref_parts(N, l.V));
     const int64_t seg = a.add(fused ? 0 : 32 * dta_pref_segs(l.B, l.S, l.V));
     a.make(z);
@@ -212,14 +212,14 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
       Tensor dz = torch::empty(z.sizes(), z.options());
       ok(dta_pref_policy_grad(l, type, temperature, p, a.at(part), loss.data_ptr<float>(),
                               stats.data_ptr<float>(), logp.data_ptr<float>(), a.at(rows),
-                              reinterpret_cast<float*>(a.at(weight)), dz.data_ptr(), st),
+                              reinterpret_cast<double*>(a.at(weight)), dz.data_ptr(), st),
          "policy_loss");
       ctx->saved_data["dz"] = dz;
       ctx->saved_data["capture"] = (int64_t)capture_of(st);
     } else {
       ok(dta_pref_policy(l, type, temperature, p, a.at(part), reinterpret_cast<double*>(a.at(seg)),
                          loss.data_ptr<float>(), stats.data_ptr<float>(), logp.data_ptr<float>(), a.at(rows),
-                         reinterpret_cast<float*>(a.at(weight)), st),
+                         reinterpret_cast<double*>(a.at(weight)), st),
          "policy_loss");
     }
     ctx->save_for_backward({z, target, a.t});
@@ -278,14 +278,14 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     const at::DeviceGuard guard(z.device());
     const int64_t N = l.B * l.S;
     Arena a;
-    const int64_t rows = a.add(16 * N), weight = a.add(4 * l.B), part = a.add(16 * dta_pref_parts(N, l.V));
+    const int64_t rows = a.add(16 * N), weight = a.add(8 * l.B), part = a.add(16 * dta_pref_parts(N, l.V));
     const int64_t seg = a.add(16 * (dta_pref_segs(l.B, l.S, l.V) + l.B));
     a.make(z);
     const auto f32 = z.options().dtype(torch::kFloat32);
     Tensor loss = torch::empty({}, f32), logp = torch::empty({l.B}, f32), margin = torch::empty({l.B / 2}, f32);
     ok(dta_pref_pairs(l, type, ref, ref_stride, beta, smoothing, average, scale, a.at(part),
                       reinterpret_cast<double*>(a.at(seg)), loss.data_ptr<float>(), logp.data_ptr<float>(),
-                      margin.data_ptr<float>(), a.at(rows), reinterpret_cast<float*>(a.at(weight)), stream_on(z)),
+                      margin.data_ptr<float>(), a.at(rows), reinterpret_cast<double*>(a.at(weight)), stream_on(z)),
        "preference_loss");
     ctx->save_for_backward({z, target, a.t});
     ctx->saved_data["ignore"] = ignore;

@@ -122,9 +122,11 @@ struct TokenArray {  // fp32 [B, S] of any strides (0: broadcast); p null where 
   __device__ __forceinline__ float at(int64_t b, int64_t s) const { return p[b * sb + s * ss]; }
 };
 
-// What the gradient needs of a row
+// What the gradient needs of a row.  coef: dloss/dlp without the sequence's weight; with the weight, the gradient that
+// arrives and 1 / temperature it is multiplied in 64 bits and rounded to fp32 once, as the product k.
 struct RowState {
-  float M, l2s, coef, pad;  // coef: dloss/dlp without the sequence's weight
+  float M, l2s;
+  double coef;
 };
 
 // A row is one workgroup's, or, where it is short (NT = 64), one wave's: four rows in a workgroup of 256 threads, which
@@ -291,13 +293,13 @@ __global__ void __launch_bounds__(256) logprob_rows_kernel(Logits L, const RowSu
   const unsigned row = blockIdx.x * (256u / lanes) + threadIdx.x / lanes;
   const bool there = row < L.B * L.S;
   const int64_t b = L.sequence_of(row), s = L.token_of(row), t = there ? L.target_of(b, s) : -1;
-  RowState st{0.f, 0.f, 0.f, 0.f};
+  RowState st{0.f, 0.f, 0.0};
   double S, lp = 0.0;
   join_pieces(part, pieces, lanes, row, t >= 0, c, &st.M, &S);
   if (!there || (threadIdx.x & (lanes - 1))) return;
   if (t >= 0) {
     lp = row_logprob((float)L.row<T>(b, s)[t], st.M, S, inv_temp, &st.l2s);
-    st.coef = 1.f;
+    st.coef = 1.0;
   }
   logp[row] = (float)lp;
   rows[row] = st;
@@ -312,6 +314,10 @@ struct PolicyArgs {
 // A value that is the same in every lane, in a scalar register
 __device__ __forceinline__ float scalar(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+__device__ __forceinline__ double scalar(double x) {
+  const int2 h = __builtin_bit_cast(int2, x);
+  return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_readfirstlane(h.x), __builtin_amdgcn_readfirstlane(h.y)));
 }
 
 struct TokenInputs {
@@ -374,7 +380,7 @@ __global__ void __launch_bounds__(NT * kRows<NT>) lse_partial_kernel(Logits L, S
   if (t < 0) {
     if (THEN == kPieces || tid != 0) return;
     if (THEN == kLogprobs || THEN == kPolicy) logp[row] = 0.f;
-    rows[row] = RowState{0.f, 0.f, 0.f, 0.f};
+    rows[row] = RowState{0.f, 0.f, 0.0};
     if (THEN == kPolicy) static_cast<double4*>(seg)[row] = make_double4(0.0, 0.0, 0.0, 0.0);
     if (THEN == kPairs) static_cast<double2*>(seg)[row] = make_double2(0.0, 0.0);
     return;
@@ -412,13 +418,13 @@ __global__ void __launch_bounds__(NT * kRows<NT>) lse_partial_kernel(Logits L, S
     part[group] = all;
     return;
   }
-  RowState st{all.M, 0.f, 1.f, 0.f};
+  RowState st{all.M, 0.f, 1.0};
   const double lp = row_logprob(zt, all.M, all.S, inv_temp, &st.l2s);
   if (THEN == kPolicy) {
     double loss, slope, kl;
     bool clipped;
     policy_token(a, in, lp, exp(lp - (double)in.old_logp), in.has_ref ? exp((double)in.ref_logp - lp) : 1.0, &loss, &slope, &kl, &clipped);
-    st.coef = (float)slope;
+    st.coef = slope;
     static_cast<double4*>(seg)[row] = make_double4(loss, kl, clipped ? 1.0 : 0.0, 1.0);
   }
   if (THEN == kPairs) static_cast<double2*>(seg)[row] = make_double2(lp, 1.0);
@@ -436,7 +442,7 @@ __global__ void __launch_bounds__(256) policy_rows_kernel(Logits L, const RowSum
   const int64_t s = (int64_t)(blockIdx.x % (unsigned)segs) * (256 / lanes) + threadIdx.x / lanes, row = b * L.S + s;
   const int64_t t = s < L.S ? L.target_of(b, s) : -1;
   double v[4] = {0.0, 0.0, 0.0, 0.0};
-  RowState st{0.f, 0.f, 0.f, 0.f};
+  RowState st{0.f, 0.f, 0.0};
   double S, lp = 0.0;
   join_pieces(part, pieces, lanes, row, t >= 0, c, &st.M, &S);
   if (s < L.S && (threadIdx.x & (lanes - 1)) == 0) {
@@ -448,7 +454,7 @@ __global__ void __launch_bounds__(256) policy_rows_kernel(Logits L, const RowSum
       policy_token(a, in, lp, exp(lp - (double)in.old_logp), in.has_ref ? exp((double)in.ref_logp - lp) : 1.0, &v[0], &slope, &v[1], &clipped);
       v[2] = clipped ? 1.0 : 0.0;
       v[3] = 1.0;
-      st.coef = (float)slope;
+      st.coef = slope;
     }
     logp[row] = (float)lp;
     rows[row] = st;
@@ -460,20 +466,20 @@ __global__ void __launch_bounds__(256) policy_rows_kernel(Logits L, const RowSum
 // stats: {kl, clip fraction}; weight[b]: what a token of sequence b counts in the loss
 __global__ void __launch_bounds__(kTotalThreads) policy_total_kernel(const double* __restrict__ seg, int64_t B, int segs,
                                                            int by_sequence, double scale, float* __restrict__ loss,
-                                                           float* __restrict__ stats, float* __restrict__ weight) {
+                                                           float* __restrict__ stats, double* __restrict__ weight) {
   double v[4] = {0.0, 0.0, 0.0, 0.0};
   for_each_sequence<4>(seg, B, segs, [&](int64_t b, double (&q)[4]) {
     if (by_sequence) {
       const double w = 1.0 / ((q[3] > 1.0 ? q[3] : 1.0) * (double)B);
       q[0] *= w;
-      weight[b] = (float)(w * scale);
+      weight[b] = w * scale;
     }
     for (int k = 0; k < 4; ++k) v[k] += q[k];
   });
   block_sums64<4, kTotalThreads / 64>(v);
   const double w = 1.0 / (v[3] > 1.0 ? v[3] : 1.0);
   if (!by_sequence)
-    for (int64_t b = threadIdx.x; b < B; b += kTotalThreads) weight[b] = (float)(w * scale);
+    for (int64_t b = threadIdx.x; b < B; b += kTotalThreads) weight[b] = w * scale;
   if (threadIdx.x == 0) {
     *loss = (float)(v[0] * (by_sequence ? scale : w * scale));
     stats[0] = (float)(v[1] * w);
@@ -491,14 +497,14 @@ __global__ void __launch_bounds__(256) pair_rows_kernel(Logits L, const RowSum* 
   const int64_t s = (int64_t)(blockIdx.x % (unsigned)segs) * (256 / lanes) + threadIdx.x / lanes, row = b * L.S + s;
   const int64_t t = s < L.S ? L.target_of(b, s) : -1;
   double v[2] = {0.0, 0.0};
-  RowState st{0.f, 0.f, 0.f, 0.f};
+  RowState st{0.f, 0.f, 0.0};
   double S;
   join_pieces(part, pieces, lanes, row, t >= 0, c, &st.M, &S);
   if (s < L.S && (threadIdx.x & (lanes - 1)) == 0) {
     if (t >= 0) {
       v[0] = row_logprob((float)L.row<T>(b, s)[t], st.M, S, 1.0, &st.l2s);
       v[1] = 1.0;
-      st.coef = 1.f;
+      st.coef = 1.0;
     }
     rows[row] = st;
   }
@@ -512,7 +518,7 @@ __global__ void __launch_bounds__(kTotalThreads) pair_total_kernel(const double*
                                                          double beta, double smoothing, int average, double scale,
                                                          double2* __restrict__ total, float* __restrict__ loss,
                                                          float* __restrict__ logp, float* __restrict__ margin,
-                                                         float* __restrict__ weight) {
+                                                         double* __restrict__ weight) {
   for_each_sequence<2>(seg, 2 * P, segs, [&](int64_t b, double (&q)[2]) {
     const double share = average ? 1.0 / (q[1] > 1.0 ? q[1] : 1.0) : 1.0;
     logp[b] = (float)(q[0] * share);
@@ -528,8 +534,8 @@ __global__ void __launch_bounds__(kTotalThreads) pair_total_kernel(const double*
     v[0] += (1.0 - smoothing) * (tail + (h < 0.0 ? -h : 0.0)) + smoothing * (tail + (h > 0.0 ? h : 0.0));
     margin[p] = (float)h;
     const double slope = scale * beta / (double)P * (1.0 / (1.0 + exp(-h)) - (1.0 - smoothing));
-    weight[p] = (float)(slope * yes.y);
-    weight[p + P] = (float)(-slope * no.y);
+    weight[p] = slope * yes.y;
+    weight[p + P] = -slope * no.y;
   }
   block_sums64<1, kTotalThreads / 64>(v);
   if (threadIdx.x == 0) *loss = (float)(scale * v[0] / (double)P);
@@ -588,8 +594,8 @@ __device__ __forceinline__ void write_zeros(T* out, int begin, int V) {
 // first, for what the forward left in the Infinity Cache, changed nothing (425 us with the forward, 417 as it is).
 template <typename T, int NT>
 __global__ void __launch_bounds__(kGradThreads) logit_grad_kernel(Logits L, Scale c, const RowState* __restrict__ rows,
-                                                                  const float* __restrict__ weight, TokenArray gout,
-                                                                  float inv_temp, int spans, int64_t units,
+                                                                  const double* __restrict__ weight, TokenArray gout,
+                                                                  double inv_temp, int spans, int64_t units,
                                                                   int unless_one, T* __restrict__ dz) {
   if (unless_one && *gout.p == 1.f) return;
   for (int64_t u = group_of<NT>(); u < units; u += gridDim.x * kRows<NT>) {
@@ -613,7 +619,7 @@ __global__ void __launch_bounds__(kGradThreads) logit_grad_kernel(Logits L, Scal
       if (cc < whole<T>(V)) r[u].load(x, cc);
     }
     const RowState st = rows[row];
-    const float k = st.coef * (weight ? weight[b] : 1.f) * gout.at(b, s0) * inv_temp;
+    const float k = (float)(st.coef * (weight ? weight[b] : 1.0) * (double)gout.at(b, s0) * inv_temp);
     write_grad<T, kGradChunks, NT>(r, out, begin, V, st.M, st.l2s, k, c);
     if (tail) out[last] = (T)grad_of((float)x[last], st.M, st.l2s, k, c);
     if (t >= begin && t - begin < kGradSpan<T, NT>)
@@ -625,7 +631,7 @@ __global__ void __launch_bounds__(kGradThreads) logit_grad_kernel(Logits L, Scal
 // A token's weight in the loss is known before its logits are read: counted first, by one workgroup.
 // weight[b] = scale / tokens, or scale / (B * tokens of b); count[0] = tokens
 __global__ void __launch_bounds__(1024) policy_weight_kernel(Logits L, int by_sequence, double scale,
-                                                             float* __restrict__ weight, double* __restrict__ count) {
+                                                             double* __restrict__ weight, double* __restrict__ count) {
   const int lane = threadIdx.x & 63;
   double v[1] = {0.0};  // of this thread
   if (by_sequence && L.B >= 16) {  // a wave a sequence
@@ -635,7 +641,7 @@ __global__ void __launch_bounds__(1024) policy_weight_kernel(Logits L, int by_se
       v[0] += (double)n;
 #pragma unroll
       for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, kWave);
-      if (lane == 0) weight[b] = (float)(scale / ((double)(n > 1 ? n : 1) * (double)L.B));
+      if (lane == 0) weight[b] = scale / ((double)(n > 1 ? n : 1) * (double)L.B);
     }
   } else if (by_sequence) {  // all of them a sequence
     for (int64_t b = 0; b < L.B; ++b) {
@@ -643,7 +649,7 @@ __global__ void __launch_bounds__(1024) policy_weight_kernel(Logits L, int by_se
       for (int64_t s = threadIdx.x; s < L.S; s += 1024) n[0] += L.target_of(b, s) >= 0 ? 1.0 : 0.0;
       v[0] += n[0];
       block_sums64<1, 16>(n);
-      if (threadIdx.x == 0) weight[b] = (float)(scale / ((n[0] > 1.0 ? n[0] : 1.0) * (double)L.B));
+      if (threadIdx.x == 0) weight[b] = scale / ((n[0] > 1.0 ? n[0] : 1.0) * (double)L.B);
     }
   } else {
     int n = 0;
@@ -659,7 +665,7 @@ __global__ void __launch_bounds__(1024) policy_weight_kernel(Logits L, int by_se
   }
   block_sums64<1, 16>(v);
   if (!by_sequence)
-    for (int64_t b = threadIdx.x; b < L.B; b += 1024) weight[b] = (float)(scale / (v[0] > 1.0 ? v[0] : 1.0));
+    for (int64_t b = threadIdx.x; b < L.B; b += 1024) weight[b] = scale / (v[0] > 1.0 ? v[0] : 1.0);
   if (threadIdx.x == 0) *count = v[0];
 }
 
@@ -700,7 +706,7 @@ __device__ __forceinline__ void add_chunks(Chunk<T> (&r)[N], int V, const Scale&
 // left is mostly the time that a row's terms keep its workgroup waiting.
 template <typename T, int NT, int CHUNKS, int WAVES>  // WAVES a SIMD that the registers leave room for
 __global__ void __launch_bounds__(NT * kRows<NT>, WAVES) policy_fused_kernel(Logits L, Scale c, double inv_temp, PolicyArgs a,
-                                                                 const float* __restrict__ weight,
+                                                                 const double* __restrict__ weight,
                                                                  float* __restrict__ logp, RowState* __restrict__ rows,
                                                                  PolicyTerms* __restrict__ terms, T* __restrict__ dz) {
   const unsigned group = group_of<NT>();
@@ -713,7 +719,7 @@ __global__ void __launch_bounds__(NT * kRows<NT>, WAVES) policy_fused_kernel(Log
     if (last < V) out[last] = (T)0.f;
     if (tid == 0) {
       logp[row] = 0.f;
-      rows[row] = RowState{0.f, 0.f, 0.f, 0.f};
+      rows[row] = RowState{0.f, 0.f, 0.0};
       terms[row] = {0.0, 0.0};
     }
     return;
@@ -721,7 +727,8 @@ __global__ void __launch_bounds__(NT * kRows<NT>, WAVES) policy_fused_kernel(Log
   const T* x = L.row<T>(b, s0);
   // what the row's terms need is requested first: thread 0 works on them while all the others wait
   TokenInputs in(a, b, s0);
-  float zt = (float)x[t], w = weight[b];
+  float zt = (float)x[t];
+  double w = weight[b];
   const float tail = last < V ? (float)x[last] : -INFINITY;
   Chunk<T> r[CHUNKS];
 #pragma unroll
@@ -744,12 +751,11 @@ __global__ void __launch_bounds__(NT * kRows<NT>, WAVES) policy_fused_kernel(Log
     double loss, slope, kl;
     bool clipped;
     policy_token(a, in, lp, __shfl(e, 0, kWave), __shfl(e, 1, kWave), &loss, &slope, &kl, &clipped);
-    const RowState st{M, l2s, (float)slope, 0.f};
-    k = st.coef * w * (float)inv_temp;
+    k = (float)(slope * w * inv_temp);
     if (tid == 0) {
       logp[row] = (float)lp;
-      rows[row] = st;
-      terms[row] = {loss * (double)w, copysign(kl, clipped ? -1.0 : 1.0)};
+      rows[row] = RowState{M, l2s, slope};
+      terms[row] = {loss * w, copysign(kl, clipped ? -1.0 : 1.0)};
     }
   }
   if constexpr (NT == 64) {  // the wave's first lane has them
@@ -927,7 +933,7 @@ static PolicyArgs policy_args(const PrefPolicy& p) {
 }
 
 hipError_t dta_pref_policy(const PrefLogits& l, int type, double temperature, const PrefPolicy& p, void* part,
-                           double* seg, float* loss, float* stats, float* logp, void* rows, float* weight,
+                           double* seg, float* loss, float* stats, float* logp, void* rows, double* weight,
                            hipStream_t st) {
   const Logits L = logits_of(l);
   const int64_t N = L.B * L.S;
@@ -960,7 +966,7 @@ int dta_pref_policy_fused(int type, int64_t N, int64_t V) {
 }
 
 template <typename T, int NT, int CHUNKS, int WAVES>
-static void policy_fused(const Logits& L, double temperature, const PrefPolicy& p, const float* weight, float* logp,
+static void policy_fused(const Logits& L, double temperature, const PrefPolicy& p, const double* weight, float* logp,
                          void* rows, void* terms, void* dz, hipStream_t st) {
   hipLaunchKernelGGL((policy_fused_kernel<T, NT, CHUNKS, WAVES>), dim3((unsigned)((L.B * L.S + kRows<NT> - 1) / kRows<NT>)),
                      dim3(NT * kRows<NT>), 0, st, L,
@@ -969,7 +975,7 @@ static void policy_fused(const Logits& L, double temperature, const PrefPolicy& 
 }
 
 hipError_t dta_pref_policy_grad(const PrefLogits& l, int type, double temperature, const PrefPolicy& p, void* terms,
-                                float* loss, float* stats, float* logp, void* rows, float* weight, void* dz,
+                                float* loss, float* stats, float* logp, void* rows, double* weight, void* dz,
                                 hipStream_t st) {
   const Logits L = logits_of(l);
   const int64_t N = L.B * L.S;
@@ -1010,7 +1016,7 @@ hipError_t dta_pref_policy_grad(const PrefLogits& l, int type, double temperatur
 
 hipError_t dta_pref_pairs(const PrefLogits& l, int type, const float* ref, int64_t ref_stride, double beta,
                           double smoothing, int average, double scale, void* part, double* seg, float* loss,
-                          float* logp, float* margin, void* rows, float* weight, hipStream_t st) {
+                          float* logp, float* margin, void* rows, double* weight, hipStream_t st) {
   const Logits L = logits_of(l);
   const int64_t N = L.B * L.S;
   const LseShape sh = lse_shape(N, L.V);
@@ -1033,13 +1039,13 @@ hipError_t dta_pref_pairs(const PrefLogits& l, int type, const float* ref, int64
   return hipGetLastError();
 }
 
-hipError_t dta_pref_grad(const PrefLogits& l, int type, double temperature, const void* rows, const float* weight,
+hipError_t dta_pref_grad(const PrefLogits& l, int type, double temperature, const void* rows, const double* weight,
                          const PrefTokens& gout, int unless_one, void* dz, hipStream_t st) {
   const Logits L = logits_of(l);
   const int64_t N = L.B * L.S;
   if (N == 0) return hipSuccess;
   DTA_BY_TYPE(type, {
-    const float inv = (float)(1.0 / temperature);
+    const double inv = 1.0 / temperature;
     // (a launch that is expected to end at once is a small one, whose workgroups walk over the rows if they have to)
     const int64_t most = unless_one ? 2048 : kMostGroups;
     if (wave_grads<T>(L)) {

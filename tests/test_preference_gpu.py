@@ -705,3 +705,38 @@ def test_small_kl(S, grad, step):
     assert abs(float(out.kl) / float(want.mean()) - 1.0) <= tol
     assert abs(float(out.loss.detach()) / (0.5 * float(want.mean())) - 1.0) <= tol + 2.0 ** -24
     assert float(out.clip_fraction) == 0.0
+
+
+@pytest.mark.parametrize("S", [9, 77, 700])
+def test_coefficients_are_rounded_once(S):
+    """Uniform rows of 1024 fp32 logits: a probability is 2^-10 exactly, so -2^10 times a gradient (not the target's) is the row's
+    coefficient, slope x weight x arriving gradient / temperature, whose one rounding to fp32 is half a step."""
+    B, V, T = 2, 1024, 0.7
+    g = torch.Generator().manual_seed(S)
+    z = torch.zeros(B, S, V, device=DEV, requires_grad=True)
+    target = torch.zeros(B, S, dtype=torch.int64, device=DEV)
+    target[1, S // 3:] = -100
+    live = (target == 0).double()
+    w, adv = torch.randn(B, S, generator=g).to(DEV), torch.randn(B, generator=g).to(DEV)
+    lp = -10.0 * math.log(2.0)
+    old = (lp + 0.1 * torch.rand(B, S, generator=g, dtype=torch.float64)).float().to(DEV)
+    tokens = live.sum(1, keepdim=True)
+
+    def near(loss, arriving, k):
+        (grad,) = torch.autograd.grad(loss, z, arriving)
+        k = k * live
+        # (fp64: the slope's exponentials and products, a few 2^-53)
+        off = (grad[..., 5].double() * -1024.0 - k).abs() - k.abs() * (2.0 ** -24 + 2.0 ** -46)
+        assert (off <= 0).all(), float((off / k.abs()).nan_to_num(0.0).max())
+
+    near(preference.token_logprobs(z, target, temperature=T), w, w.double() / T)
+    r = torch.exp(lp - old.double())
+    out = preference.policy_loss(z, target, old, adv, reduction="sequence", temperature=T, scale=0.3, clip=0.9)
+    near(out.loss, None, -r * adv.double()[:, None] * 0.3 / T / tokens / B)
+    out = preference.policy_loss(z, target, old, adv, reduction="sequence", temperature=T, scale=0.3, clip=0.9)
+    arriving = torch.tensor(0.77, device=DEV)
+    near(out.loss, arriving, -r * adv.double()[:, None] * 0.3 / T * arriving.double() / tokens / B)
+    pair = preference.preference_loss(z, target, torch.tensor([0.3, -0.4], device=DEV), beta=0.37, average=True, scale=0.3)
+    h = 0.37 * -(torch.tensor(0.3).double() + torch.tensor(0.4).double()).item()
+    slope = 0.3 * 0.37 * (1.0 / (1.0 + math.exp(-h)) - 1.0)
+    near(pair.loss, None, torch.tensor([[slope], [-slope]], device=DEV, dtype=torch.float64) / tokens)
