@@ -8,14 +8,14 @@ a position does not count (prompts, padding).  Positions that do not count -- a 
 
 GPU tensors take the HIP kernels of ``csrc/preference.hip`` (bf16, fp16 or fp32 logits; rows of any stride and
 alignment, any vocabulary) through the autograd functions of ``csrc/bindings_pref.cpp``, which check their tensors.
-CPU tensors take the same math in PyTorch.  Per-token inputs are fp32; statistics over the vocabulary are fp32,
-per-token terms and sums fp64.  On the GPU each loss can be differentiated once: a gradient taken with ``create_graph`` is
-refused where it is differentiated itself.
+CPU tensors take the same math in PyTorch, fp64 logits among them (with fp32 or fp64 per-token inputs).  Beside other
+logits per-token inputs are fp32; statistics over the vocabulary are fp32, per-token terms and sums fp64.  On the GPU
+each loss can be differentiated once: a gradient taken with ``create_graph`` is refused where it is differentiated.
 """
 from __future__ import annotations
 
 import math
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 import torch.nn.functional as F
@@ -58,16 +58,16 @@ def _check(logits: torch.Tensor, target: torch.Tensor) -> None:
         raise TypeError(f"logits must be floating point (got {logits.dtype})")
 
 
-def _check_tokens(t: Optional[torch.Tensor], target: torch.Tensor, name: str, per_sequence: bool = False) -> None:
+def _check_tokens(t: Optional[torch.Tensor], logits: torch.Tensor, name: str, shapes: Sequence[torch.Size]) -> None:
     if t is None:
         return
-    shapes = [target.shape] + ([target.shape[:1]] if per_sequence and target.dim() == 2 else [])
     if t.shape not in shapes:
         raise ValueError(f"{name} must be {' or '.join(str(tuple(s)) for s in shapes)} (got {tuple(t.shape)})")
-    if t.dtype not in (torch.float32, torch.float64):
-        raise TypeError(f"{name} must be float32 (got {t.dtype})")
-    if t.device != target.device:
-        raise ValueError(f"{name} is on {t.device}, logits on {target.device}")
+    # (fp64 logits, which only the CPU takes, have fp64 log-probabilities)
+    if t.dtype != torch.float32 and not (t.dtype == logits.dtype == torch.float64):
+        raise TypeError(f"{name} must be float32 (got {t.dtype}, logits {logits.dtype})")
+    if t.device != logits.device:
+        raise ValueError(f"{name} is on {t.device}, logits on {logits.device}")
 
 
 def _positive(x: float, name: str) -> float:
@@ -180,8 +180,8 @@ def policy_loss(logits: torch.Tensor, target: torch.Tensor, old_logp: torch.Tens
                                                 reduction == "sequence", ignore_index, temperature, scale))
     _check(logits, target)
     for t, name in ((old_logp, "old_logp"), (ref_logp, "ref_logp")):
-        _check_tokens(t, target, name)
-    _check_tokens(advantages, target, "advantages", per_sequence=True)
+        _check_tokens(t, logits, name, [target.shape])
+    _check_tokens(advantages, logits, "advantages", [target.shape, target.shape[:1]][:target.dim()])
     return policy_loss_reference(logits, target, old_logp.detach(), advantages.detach(),
                                  None if ref_logp is None else ref_logp.detach(), clip, clip_high, kl_coef, reduction,
                                  ignore_index, temperature, scale)
@@ -228,9 +228,6 @@ def preference_loss(logits: torch.Tensor, target: torch.Tensor, ref_logp: Option
     if logits.dim() != 3 or logits.shape[0] < 2 or logits.shape[0] % 2:
         raise ValueError("logits must be [2 P, S, V]: P chosen sequences, then as many rejected ones "
                          f"(got {tuple(logits.shape)})")
-    if ref_logp is not None:
-        if ref_logp.shape != logits.shape[:1]:
-            raise ValueError(f"ref_logp must be {tuple(logits.shape[:1])} (got {tuple(ref_logp.shape)})")
-        _check_tokens(ref_logp, target[:, 0] if target.shape[1] else ref_logp, "ref_logp")
-        ref_logp = ref_logp.detach()
+    _check_tokens(ref_logp, logits, "ref_logp", [logits.shape[:1]])
+    ref_logp = None if ref_logp is None else ref_logp.detach()
     return preference_loss_reference(logits, target, ref_logp, beta, label_smoothing, average, ignore_index, scale)

@@ -302,3 +302,23 @@ def test_the_trainer_clips_complex_gradients():
     for a, b in zip(nets[0].parameters(), nets[1].parameters()):
         # torch's fp32 norm of 8 numbers, and the step's own subtraction
         torch.testing.assert_close(a, b, rtol=16 * 2.0 ** -24, atol=16 * 2.0 ** -24 * 0.1)
+
+
+def test_per_token_inputs_are_fp32_on_every_device():
+    """What the GPU refuses (fp64 per-token inputs beside fp32 or 16-bit logits) the CPU refuses too; fp64 logits, which only the
+    CPU takes, come with either."""
+    z, target, old, ref, adv = _inputs()
+    P, R = preference.policy_loss, preference.preference_loss
+    for dtype in (torch.float32, torch.bfloat16):
+        x = z.to(dtype)
+        P(x, target, old.float(), adv.float(), ref.float())
+        for bad in ([old, adv.float(), ref.float()], [old.float(), adv, ref.float()], [old.float(), adv.float(), ref],
+                    [old.float(), adv[:, 0], ref.float()]):
+            with pytest.raises(TypeError, match="must be float32"):
+                P(x, target, *bad)
+        R(x, target, ref[:, 0].float())
+        with pytest.raises(TypeError, match="ref_logp must be float32"):
+            R(x, target, ref[:, 0])
+    a, b = P(z, target, old.float(), adv.float(), ref.float()), P(z, target, old, adv, ref)
+    assert a.loss.dtype == b.loss.dtype == torch.float64
+    R(z[:, :0], target[:, :0], ref[:, 0])
