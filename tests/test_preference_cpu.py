@@ -333,7 +333,9 @@ def test_norm_on_the_host_takes_no_copies():
     before = resource.getrusage(resource.RUSAGE_SELF).ru_maxrss
     norm = optim.clip_grads_([g], 2.5)
     assert resource.getrusage(resource.RUSAGE_SELF).ru_maxrss - before < 128 << 10  # KiB
-    assert float(norm) == 5.0 and float(g[5]) == 1.5 and float(g[-1]) == 2.0
+    coef = 2.5 / (5.0 + 1e-6)  # (rounded to fp32, and the products)
+    assert float(norm) == 5.0
+    assert abs(float(g[5]) / (3.0 * coef) - 1) <= 2.0 ** -23 and abs(float(g[-1]) / (4.0 * coef) - 1) <= 2.0 ** -23
     n = (1 << 18) * 2 + 3  # pieces and a remainder, strided, fp64 (read as it is, not squared in place)
     for t in (torch.randn(n, generator=torch.Generator().manual_seed(0)), torch.randn(n, 2).double()[:, 1]):
         keep = t.clone()
