@@ -93,14 +93,25 @@ __device__ __forceinline__ double sumsq_unit(const T* __restrict__ p, int64_t c0
   return acc;
 }
 
-// The coefficient is used in fp32 (2^-24 relative; fp64 gradients take it whole) and each product rounded to T
+// The coefficient is used in fp32 (2^-24 relative; fp64 gradients take it whole) and each product rounded to T.  Below
+// fp32's normal numbers (gradients near 1e38) it would lose bits: it is held 2^64 times as large there, and `rest` takes
+// the product back (exactly, or with the one rounding of a subnormal product).
+struct Coef {
+  double whole;
+  float f, rest;
+  __device__ __forceinline__ explicit Coef(double c) : whole(c) {
+    const bool tiny = c < 0x1p-126;
+    f = (float)(tiny ? c * 0x1p64 : c);
+    rest = tiny ? 0x1p-64f : 1.f;
+  }
+};
 template <typename T>
-__device__ __forceinline__ T scaled(T x, double coef) {
-  if constexpr (sizeof(T) == 8) return x * coef;
-  else return (T)((float)x * (float)coef);
+__device__ __forceinline__ T scaled(T x, const Coef& c) {
+  if constexpr (sizeof(T) == 8) return x * c.whole;
+  else return (T)((float)x * c.f * c.rest);
 }
 template <typename T>
-__device__ __forceinline__ void scale_unit(T* __restrict__ p, int64_t c0, int64_t numel, double coef) {
+__device__ __forceinline__ void scale_unit(T* __restrict__ p, int64_t c0, int64_t numel, const Coef& coef) {
   constexpr int W = Pack<T>::n, STEP = 256 * W, LOADS = kUnit / STEP, U = LOADS < 4 ? LOADS : 4;
   if (c0 + kUnit <= numel) {
     for (int l = 0; l < LOADS; l += U) {
@@ -207,8 +218,9 @@ __global__ void __launch_bounds__(1024) grad_norm_kernel(const double* __restric
 // A norm within the bound leaves every gradient as it is: the workgroups end without touching them.  A NaN norm
 // gives a NaN coefficient (not 1), an infinite one 0, as min(1, max_norm / (norm + 1e-6)) says.
 __device__ __forceinline__ void clip_units(const NormJobs& jobs, double root, double max_norm) {
-  const double coef = max_norm / (root + 1e-6);
-  if (coef >= 1.0) return;
+  const double c = max_norm / (root + 1e-6);
+  if (c >= 1.0) return;
+  const Coef coef(c);
   walk_units<true>(jobs, [&](void* p, int type, int64_t c0, int64_t numel, bool) {
     if (type == 1) scale_unit((bf16*)p, c0, numel, coef);
     else if (type == 0) scale_unit((float*)p, c0, numel, coef);
@@ -251,7 +263,7 @@ __device__ __forceinline__ double small_sumsq(const T* p, int64_t c0, int64_t nu
   return acc;
 }
 template <typename T>
-__device__ __forceinline__ void small_scale(T* p, int64_t c0, int64_t numel, double coef) {
+__device__ __forceinline__ void small_scale(T* p, int64_t c0, int64_t numel, const Coef& coef) {
 #pragma unroll
   for (int k = 0; k < kSmallUnit / 64; ++k) {
     const int64_t i = c0 + k * 64 + (threadIdx.x & 63);
@@ -277,8 +289,9 @@ __global__ void __launch_bounds__(1024) grad_clip_small_kernel(NormJobs jobs, do
   });
   const double root = sqrt(block_sum64<1024>(acc));
   if (threadIdx.x == 0) *norm = (float)root;
-  const double coef = max_norm / (root + 1e-6);
-  if (coef >= 1.0) return;
+  const double c = max_norm / (root + 1e-6);
+  if (c >= 1.0) return;
+  const Coef coef(c);
   walk([&](void* p, int type, int64_t c0, int64_t numel) {
     if (type == 1) small_scale((bf16*)p, c0, numel, coef);
     else if (type == 0) small_scale((float*)p, c0, numel, coef);

@@ -102,8 +102,14 @@ def grad_clip_(tensors: Iterable[torch.Tensor], sumsq: torch.Tensor, max_norm: f
     for device, ts in _by_device(tensors).items():
         if device.type != "cuda":
             coef = (float(max_norm) / (sumsq.to(device).sqrt() + 1e-6)).clamp(max=1.0)
+            tiny = float(coef) < 2.0 ** -126  # (in fp32 it would lose bits: 2^64 times as large, and the products back)
             for t in ts:
-                t.mul_(coef.to(t.dtype) if t.dtype == torch.float64 else coef.float())
+                if t.dtype == torch.float64:
+                    t.mul_(coef)
+                elif tiny:
+                    t.mul_((coef * 2.0 ** 64).float()).mul_(2.0 ** -64)
+                else:
+                    t.mul_(coef.float())
             continue
         flat = [t if _fills_memory(t) else t.contiguous() for t in ts]
         native().grad_clip_(flat, sumsq.to(device), float(max_norm))

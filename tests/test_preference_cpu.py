@@ -341,3 +341,20 @@ def test_norm_on_the_host_takes_no_copies():
         keep = t.clone()
         want = math.sqrt(float(t.double().square().sum()))
         assert abs(float(optim.global_norm(t)) - want) <= 2.0 ** -23 * want and torch.equal(t, keep)
+
+
+def test_a_coefficient_below_fp32():
+    """Gradients near 1e37 clipped to a norm near 1 and below: the coefficient leaves fp32's normal numbers, the products do not.
+    (fp32 coefficient and product, the sum of squares in 64 bits: 2^-24 each, and half a step of the type.)"""
+    for dtype in (torch.float32, torch.bfloat16, torch.float64):
+        for n in (100, 300007):
+            base = (torch.rand(n, generator=torch.Generator().manual_seed(n)) + 0.5) * 1e37
+            p = torch.nn.Parameter(torch.zeros(n, dtype=dtype, device="cpu"))
+            before = base.to(dtype).to("cpu")
+            norm = math.sqrt(float(before.double().square().sum()))
+            for max_norm in (1.0, 1e-4):
+                p.grad = before.clone()
+                optim.clip_grad_norm_(p, max_norm)
+                want = before.double() * (max_norm / (norm + 1e-6))
+                step = 2.0 ** -40 if dtype == torch.float64 else oracle.half_step(dtype) * 1.01 + 3 * 2.0 ** -24
+                assert ((p.grad.double() - want).abs() <= want * step).all(), (dtype, n, max_norm)
