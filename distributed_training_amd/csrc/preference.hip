@@ -590,8 +590,8 @@ __device__ __forceinline__ void write_zeros(T* out, int begin, int V) {
 
 // k = coef * weight[b] * gout[b, s] / temperature (weight absent: 1; a scalar gout has strides 0).  unless_one: dz was
 // written in the forward for gout = 1, so nothing is left to do where that is what came.  Bound by the read and the write:
-// 6.4 TB/s at 8192 x 50304 bf16 (256 us), 6.2 at 1999 x 128256 fp32 (332 us).  Reading the rows from the last to the
-// first, for what the forward left in the Infinity Cache, changed nothing (425 us with the forward, 417 as it is).
+// 6.4 TB/s at 8192 x 50304 bf16 (256 us), 6.2 at 1999 x 128256 fp32 (332 us).  The forward reads with non-temporal loads,
+// so that this read finds nothing cached, in whatever order it walks the rows.
 template <typename T, int NT>
 __global__ void __launch_bounds__(kGradThreads) logit_grad_kernel(Logits L, Scale c, const RowState* __restrict__ rows,
                                                                   const double* __restrict__ weight, TokenArray gout,
@@ -801,10 +801,10 @@ struct LseShape {
   int pieces, lanes, span;
 };
 
-// Pieces of a row: up to 1024 workgroups where rows are few, each piece at least 8192 logits; lanes that join them: the
-// next power of two.  Policy loss with its gradient, bf16, in us with pieces / in one piece: 1 row of 128256 13.5 / 29.5,
-// 64 rows of 50304 17.8 / 21.8, 512 rows of 50304 39.1 / 39.2; pieces of 2048 logits 19.8 for 64 rows of 50304, and 19.1
-// instead of 16.2 for 512 rows of 8000.
+// Pieces of a row, for the few and long rows that are cut at all (in_one_piece): up to 1024 workgroups, each piece at least
+// 8192 logits; lanes that join them: the next power of two.  Log-probabilities, bf16, in us with pieces of at least 2048 /
+// 8192 / 16384 logits: 1 row of 70001 5.7 / 5.7 / 6.2, 16 of 128256 7.2 / 6.8 / 7.4, 64 of 128256 8.6 / 8.6 / 8.9, 16 of
+// 600001 10.7 / 10.7 / 10.3; the policy loss with its gradient, 16 rows of 70001 17.4 / 16.6 / 16.8.
 static LseShape lse_shape(int64_t N, int64_t V) {
   const int64_t least = 8192;
   int64_t pieces = N > 0 ? 1024 / N : 1;
@@ -834,7 +834,8 @@ static bool wave_grads(const Logits& L) { return L.B * L.S >= kWaveRows && L.V <
 static bool long_rows(const Logits& L) { return L.V > 60000 && L.B * L.S < (1 << 22); }
 // Few rows: 1024 threads a row in one launch rather than pieces and a second launch to join them,
 // unless the row is too long for that.  Pieces / one, bf16: 64 rows of 16000 5.1 / 4.3 us, of 50304 6.3 / 6.6 (with the
-// host 8.8 / 6.7), of 128256 7.9 / 11.2; 256 rows of 50304 8.9 / 7.4, of 128256 13.4 / 12.7.
+// host 8.8 / 6.7), of 128256 8.6 / 11.5; 16 of 70001 6.3 / 7.9; 1 of 600001 6.9 / 37.5; 128 of 128256 11.6 / 11.6, 255 15.4
+// / 13.4.
 static bool in_one_piece(int64_t N, int64_t V) { return lse_shape(N, V).pieces == 1 || V <= 65536 || N >= 256; }
 // The losses' terms by row, in the rows' own kernel, and added up by one workgroup: few rows, where a launch less counts (a
 // pass over pairs of 132 rows of 50257 62 -> 56.5 us, policy of 64 rows of 1003 64 -> 57.7).  With many the sums cost more than
@@ -983,9 +984,19 @@ hipError_t dta_pref_policy_grad(const PrefLogits& l, int type, double temperatur
   double* count = (double*)((PolicyTerms*)terms + N);
   hipLaunchKernelGGL(policy_weight_kernel, dim3(1), dim3(1024), 0, st, L, p.by_sequence, p.scale, weight, count);
   DTA_HIP_CHECK(hipGetLastError());
-  // Threads and 16-byte chunks a thread by the row's size: as many rows on a CU as its registers hold (V = 50304 in bf16:
-  // 1024 x 7 at 8 waves a SIMD 279 us, 512 x 13 287, 256 x 25 306, 1024 x 7 at 4 waves 367, for 8192 rows).  A wave a row
-  // for the shortest: 24000 rows of 2000 in bf16 64 x 4 38.5 us, 256 x 2 51.2; of 4000 64 x 8 69.8, 256 x 2 67.8.
+  // Threads and 16-byte chunks a thread by the row's size: as many rows on a CU as its registers hold, few lanes idle.
+  // Each form / the next one, in us of the kernel, bf16 (fp16's layout; fp32 in brackets):
+  //   64 x 2   24000 rows of 1021 31.5 / 32.6, 8000 of 500 12.6 / 13.1 (24000 of 509 24.3 / 24.3)
+  //   64 x 4   24000 of 2045 42.4 / 60.8, 2000 9.4 / 11.0, 128 7.4 / 6.5 (24000 of 1021 39.4 / 49.5)
+  //   256 x 2  24000 of 4093 78.4 / 82.8 (2045: 68.4 / 68.6)
+  //   256 x 4  24000 of 4608 82.0 / 118, of 8189 151 / 160 (2304: 73.7 / 97.6; 4093: 136 / 131)
+  //   512 x 4  24000 of 9216 159 / 237, of 16381 318 / 349 (4608: 143 / 193)
+  //   1024 x 4 24000 of 18432 337 / 342, 512 12.4 / 13.8 (512 of 9216 10.6 / 12.3)
+  //   1024 x 7 13481 of 35840 318 / 318, a pass over 8192 of 50304, 3/4 counting, 275 / 279 (14211 of 17000 334 / 345); its 64
+  //            registers spill 9, at 4 waves a SIMD without spilling 367 where 8 waves took 279
+  //   512 x 16 8278 of 58368 346 / 379, 7373 of 65533 403 / 449 (29184: 349 / 336; 512 of them 22.1 / 27.6)
+  //   1024 x 10 7149 of 67584 356 / 375, 5898 of 81917 458 / 469 (33792: 326 / 332)
+  //   1024 x 16 the rest; 1024 x 13 in between gained 2.4 % at most (5685 of 84992 364 / 373) and is left out
 #define DTA_FUSED(T, NT, CHUNKS, WAVES) \
   policy_fused<T, NT, CHUNKS, WAVES>(L, temperature, p, weight, logp, rows, terms, dz, st)
 #define DTA_FUSED_ANY(T, W)                                   \
@@ -998,7 +1009,6 @@ hipError_t dta_pref_policy_grad(const PrefLogits& l, int type, double temperatur
   else if (L.V <= W * 1024 * 7) DTA_FUSED(T, 1024, 7, 8);     \
   else if (L.V <= W * 512 * 16) DTA_FUSED(T, 512, 16, 4);     \
   else if (L.V <= W * 1024 * 10) DTA_FUSED(T, 1024, 10, 4);   \
-  else if (L.V <= W * 1024 * 13) DTA_FUSED(T, 1024, 13, 4);   \
   else DTA_FUSED(T, 1024, 16, 4);
   if (type == 1) {
     DTA_FUSED_ANY(bf16, 8)
