@@ -207,6 +207,59 @@ def test_clip_grad_norm_global(strategy):
     run_gloo(_clip_parity, 2, strategy)
 
 
+def _preference_losses(rank, ws, strategy):
+    """The preference losses behind the engines: every rank scores its own samples, and clipped gradients and the step are those of
+    one process over the mean of the ranks' losses."""
+    from distributed_training_amd.ops.optim import clip_grad_norm_
+    from distributed_training_amd.ops.preference import policy_loss, preference_loss, token_logprobs
+    from distributed_training_amd.parallel.comm import TorchComm
+    from distributed_training_amd.parallel.ddp import DistributedDataParallel
+    from distributed_training_amd.parallel.fsdp import FullyShardedDataParallel
+
+    torch.manual_seed(0)
+    V = 23
+    ref = nn.Sequential(nn.Embedding(V, 16), Block(16), Block(16), nn.Linear(16, V))
+    m = copy.deepcopy(ref)
+    if strategy == "fsdp":
+        w = FullyShardedDataParallel(m, TorchComm(), torch.device("cpu"), wrap_policy={Block})
+    else:
+        w = DistributedDataParallel(m, TorchComm())
+    g = torch.Generator().manual_seed(3)
+    idx = torch.randint(V, (ws, 4, 9), generator=g)
+    target = torch.randint(V, (ws, 4, 9), generator=g)
+    target[..., :2] = -100
+    target[0, 1, 4:] = -100
+    adv = torch.randn(ws, 4, generator=g)
+    with torch.no_grad():
+        old = [token_logprobs(ref(idx[r]), target[r]) - 0.05 for r in range(ws)]
+
+    def loss_of(model, r):
+        z = model(idx[r])
+        return (policy_loss(z, target[r], old[r], adv[r], old[r], kl_coef=0.1, reduction="sequence").loss
+                + preference_loss(z, target[r], old[r].sum(1)).loss)
+
+    o1, o2 = torch.optim.SGD(ref.parameters(), lr=1.0), torch.optim.SGD(w.parameters(), lr=1.0)
+    for _ in range(2):
+        o1.zero_grad()
+        o2.zero_grad()
+        (sum(loss_of(ref, r) for r in range(ws)) / ws).backward()
+        loss_of(w, rank).backward()
+        want, got = clip_grad_norm_(ref.parameters(), 0.05), w.clip_grad_norm_(0.05)
+        assert float(want) > 0.05
+        torch.testing.assert_close(got, want, rtol=1e-5, atol=1e-6)
+        o1.step()
+        o2.step()
+    sd = w.full_state_dict(rank0_only=False) if strategy == "fsdp" else {
+        k[len("module."):]: v for k, v in w.state_dict().items()}
+    for k, v in ref.state_dict().items():
+        torch.testing.assert_close(sd[k], v, rtol=1e-5, atol=1e-6, msg=k)
+
+
+@pytest.mark.parametrize("strategy", ["fsdp", "ddp"])
+def test_preference_losses_behind_the_engines(strategy):
+    run_gloo(_preference_losses, 2, strategy)
+
+
 def _clip_range(rank, ws):
     """Gradients whose squares leave fp32's range, of nothing, and non-finite ones: the norm over the ranks' shards."""
     from types import SimpleNamespace

@@ -740,3 +740,107 @@ def test_coefficients_are_rounded_once(S):
     h = 0.37 * -(torch.tensor(0.3).double() + torch.tensor(0.4).double()).item()
     slope = 0.3 * 0.37 * (1.0 / (1.0 + math.exp(-h)) - 1.0)
     near(pair.loss, None, torch.tensor([[slope], [-slope]], device=DEV, dtype=torch.float64) / tokens)
+
+
+@pytest.mark.parametrize("S", [12, 130])  # few rows, and enough for the policy loss's one-pass form
+def test_captured_with_a_retained_and_scaled_backward(S):
+    """One graph with a forward, a backward of a scaled loss that retains it, and another of it: every replay as the eager calls;
+    and a graph of a backward alone, whose forward ran before on the same stream."""
+    shape = (4, S, 2003)
+    fixed = [t.clone() for t in _case(*shape, torch.bfloat16)]
+    factor = torch.full((), 4.0, device=DEV)
+
+    def both(z, target, old, ref, adv, factor):
+        z = z.detach().requires_grad_()
+        loss = preference.policy_loss(z, target, old, adv, ref, kl_coef=0.1).loss
+        (a,) = torch.autograd.grad(loss, z, factor, retain_graph=True)
+        (b,) = torch.autograd.grad(loss, z)
+        return loss.detach(), a, b
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both(*fixed, factor)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both(*fixed, factor)
+    for seed in range(1, 5):
+        new = _case(*shape, torch.bfloat16, seed=seed)
+        scale = torch.full((), 0.5 if seed % 2 else 1.0, device=DEV)
+        want = both(*new, scale)
+        for f, n in zip([*fixed, factor], [*new, scale]):
+            f.copy_(n)
+        out[1].zero_(), out[2].zero_()  # (the gradients are the caller's)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+        del want, new
+    # (a power of two scales the rounded gradient exactly)
+    assert torch.equal(out[1], out[2])
+
+    z, target, old, ref, adv = _case(*shape, torch.bfloat16)
+    z.requires_grad_()
+    (want,) = torch.autograd.grad(preference.policy_loss(z, target, old, adv, ref, kl_coef=0.1).loss, z)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        loss = preference.policy_loss(z, target, old, adv, ref, kl_coef=0.1).loss
+    side.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        (got,) = torch.autograd.grad(loss, z, retain_graph=True)
+    for _ in range(3):
+        got.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    (again,) = torch.autograd.grad(loss, z)  # the eager backward of the same loss
+    assert torch.equal(again, want)
+
+
+def test_a_preference_step_under_fsdp():
+    """The losses behind the FSDP engine: gradients against the same run with the losses in 64 bits, the clip over its shards,
+    an optimizer step."""
+    from distributed_training_amd.models.gpt2 import GPT2, GPT2Config
+    from distributed_training_amd.ops.optim import FusedAdamW
+    from distributed_training_amd.parallel.comm import RcclComm
+    from distributed_training_amd.parallel.fsdp import FullyShardedDataParallel, lm_wrap_policy
+
+    torch.manual_seed(0)
+    dev = torch.device(DEV, 0)
+    model = GPT2(GPT2Config(n_layer=2, n_head=2, n_embd=128, vocab_size=1000, block_size=64)).to(dev)
+    w = FullyShardedDataParallel(model, comm=RcclComm(0, 1, dev), device=dev, wrap_policy=lm_wrap_policy(model),
+                                 param_dtype=torch.bfloat16)
+    opt = FusedAdamW(w.parameters(), lr=1e-3)
+    idx = torch.randint(1000, (4, 64), device=DEV)
+    target = torch.roll(idx, -1, 1)
+    target[:, :8] = -100
+    target[:, -1] = -100
+    adv = torch.tensor([1.0, -0.5, 0.8, -1.2], device=DEV)
+    with torch.no_grad():
+        ref_tok = preference.token_logprobs(w(idx), target)
+    for step in range(2):
+        grads = []
+        for exact in (True, False):
+            w.zero_grad(set_to_none=True)
+            logits = w(idx)
+            if exact:
+                z = logits.double()
+                loss = (oracle.policy64(z, target, ref_tok + 0.1, adv, ref_tok, kl_coef=0.05)[0]
+                        + oracle.pairs64(z, target, ref_tok.sum(1))[0]).float()
+            else:
+                loss = (preference.policy_loss(logits, target, ref_tok + 0.1, adv, ref_tok, kl_coef=0.05).loss
+                        + preference.preference_loss(logits, target, ref_tok.sum(1)).loss)
+            loss.backward()
+            torch.cuda.synchronize()
+            grads.append(w.shards.grad.double().clone())
+        a, b = grads
+        # bf16 logit gradients of two losses, rounded before their sum, and the 2 layers' roundings behind them, as under DDP
+        assert a.norm() > 0 and (a - b).norm() <= 16 * 2.0 ** -9 * a.norm() + 1e-6
+        want = float(b.norm())
+        norm = w.clip_grad_norm_(0.1)
+        assert want > 0.1 and abs(float(norm) - want) <= 2.0 ** -23 * want
+        g = b * (0.1 / (want + 1e-6))
+        assert ((w.shards.grad.double() - g).abs() <= g.abs() * (oracle.half_step(w.shards.grad.dtype) + 2.0 ** -22)).all()
+        opt.step()
+    assert all(torch.isfinite(p).all() for p in w.parameters())
