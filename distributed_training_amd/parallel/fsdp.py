@@ -954,8 +954,8 @@ class FullyShardedDataParallel(nn.Module):
 
     def clip_grad_norm_(self, max_norm: float) -> torch.Tensor:
         """Global-norm clip across the shards (torch FSDP's ``clip_grad_norm_``): the
-        squared norms of every rank's gradient shard are all-reduced before the
-        coefficient is formed, so all ranks scale by the same factor."""
+        squared norms of every rank's gradient shard are gathered and added in 64 bits
+        before the coefficient is formed, so all ranks scale by the same factor."""
         from .flat import clip_flat_grad_norm_
 
         return clip_flat_grad_norm_(self.shards, max_norm, comm=self.comm, sharded=True)
